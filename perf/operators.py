@@ -113,12 +113,14 @@ def _cache_shape(case, n_seq, rows, n_pages):
 
 # --------------------------------------------------------------- 4-bit rows
 def _quantise(x):
-    """bf16 values [..., hd] to (codes [..., hd / 2] uint8, scales [..., hd / 64] bf16): per group of 64, scale =
-    amax / 7 rounded to bf16, code = x / scale to the nearest (even) integer in -7..7, plus 7; low nibble first."""
+    """bf16 values [..., hd] to (codes [..., hd / 2] uint8, scales [..., hd / 64] bf16), the rule of the int4 weights:
+    per group of 64, scale = amax / 7 rounded to bf16 (1 where that is 0), code = x / scale to the nearest integer,
+    halves away from zero, in -7..7, plus 7; low nibble first."""
     v = x.float().unflatten(-1, (-1, GROUP))
     scale = (v.abs().amax(-1) / 7.0).to(torch.bfloat16)
-    s = scale.float().unsqueeze(-1)
-    c = torch.where(s > 0, torch.round(v / s), torch.zeros_like(v)).clamp(-7, 7) + 7
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    r = v / scale.float().unsqueeze(-1)
+    c = torch.trunc(r + torch.where(r < 0, -0.5, 0.5)).clamp(-7, 7) + 7
     c = c.flatten(-2).to(torch.uint8)
     return c[..., 0::2] | (c[..., 1::2] << 4), scale
 
@@ -386,9 +388,8 @@ def _exact_append(s):
     for name in ("k", "v"):
         x = s[name].double().reshape(s["rows"], -1, GROUP)
         scale = (x.abs().max(2, keepdim=True).values / 7).to(torch.bfloat16).double()
-        q = torch.zeros_like(x)
-        torch.div(x, scale, out=q)
-        q = torch.nan_to_num(torch.round(q), nan=0.0).clamp(-7, 7)
+        scale = torch.where(scale == 0, 1.0, scale)
+        q = torch.sign(x) * torch.floor(x.abs() / scale + 0.5).clamp(max=7)
         out[name] = (q * scale).reshape(s["rows"], -1)
     return out
 

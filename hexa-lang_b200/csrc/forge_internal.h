@@ -257,3 +257,6 @@ int forge_flash_prefill_kv(const uint16_t* q, const uint16_t* kc, const uint16_t
                            int Hkv, int S, int hd, int kv_ld, int64_t kv_rows, cudaStream_t stream);
 // v2 FLASH_PREFILL family.
 int forge_prefill_dispatch(const ForgeShapeInfo* s, const ForgeArgs* in, const ForgeArgs* out);
+// Shape and alignment checks of a 4-bit cache descriptor (kv4.cu).
+struct ForgeKv4;
+int forge_kv4_check(const ForgeKv4* c, const char* what);

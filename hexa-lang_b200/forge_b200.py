@@ -20,6 +20,7 @@ LIB_PATH = os.environ.get("FORGE_B200_LIB") or os.path.join(HERE, "libforge_b200
 
 FORGE_WEIGHT_BF16 = 0
 FORGE_WEIGHT_Q4_G128 = 1
+FORGE_LOGITS_F32, FORGE_LOGITS_BF16 = 0, 1
 FORGE_PERM_NONE, FORGE_PERM_QKV, FORGE_PERM_GATEUP = 0, 1, 2
 
 
@@ -53,6 +54,13 @@ class ForgePagedKvStats(C.Structure):
     _fields_ = [("num_pages", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32),
                 ("used_pages", C.c_int32), ("free_pages", C.c_int32), ("seq_count", C.c_int32),
                 ("stat_alloc", C.c_int64), ("stat_release", C.c_int64), ("stat_reuse", C.c_int64)]
+
+
+class ForgeKv4(C.Structure):
+    """Descriptor of a 4-bit KV cache (include/forge_kv4.h): device addresses and shape."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ks", C.c_void_p), ("vs", C.c_void_p), ("table", C.c_void_p),
+                ("n_seq", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("lmax", C.c_int32),
+                ("page_tokens", C.c_int32), ("max_pages", C.c_int32), ("num_pages", C.c_int32)]
 
 
 class ForgeClmBlock(C.Structure):
@@ -285,6 +293,13 @@ def lib() -> C.CDLL:
             "forge_paged_kv_page_table": (i32, [vp, i64, vp, i32]),
             "forge_paged_kv_stats": (i32, [vp, C.POINTER(ForgePagedKvStats)]),
             "forge_flash_decode_paged": (i32, [vp, vp, vp, i32, vp, i32, i32, vp, i32, i32, i32, i32, vp, vp, vp]),
+            "forge_kv4_append": (i32, [C.POINTER(ForgeKv4), vp, vp, i64, vp, vp, i32, vp]),
+            "forge_kv4_read": (i32, [C.POINTER(ForgeKv4), vp, vp, i32, vp, vp, i64, vp]),
+            "forge_flash_decode_kv4_workspace_bytes": (i64, [i32, i32, i32, i32]),
+            "forge_flash_decode_kv4": (i32, [vp, C.POINTER(ForgeKv4), vp, vp, i32, i32, vp, vp, vp]),
+            "forge_flash_prefill_varlen": (i32, [vp, i64, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32, vp, i64, vp,
+                                                 vp]),
+            "forge_token_logprobs": (i32, [vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]),
             "forge_clm_open": (i32, [C.c_char_p, C.POINTER(vp)]),
             "forge_clm_close": (None, [vp]),
             "forge_clm_count": (i32, [vp]),

@@ -292,6 +292,30 @@ int forge_flash_decode_noalloc_status(void);
 int forge_sample(const float* logits, int64_t ld, int batch, int vocab, double temperature, int top_k,
                  double top_p, int64_t* rng_state, float* probs, int32_t* tokens, void* stream);
 
+/* Log probabilities beside the sampler (an API's logprobs, the scoring of a
+ * prompt), one pass over the logits: rows of vocab logits, ld elements from
+ * row to row, fp32 or bf16. Per row, with p = softmax(z):
+ *   logprob [rows]   log p[tokens[r]]; 0 where tokens[r] < 0 (no token); a
+ *                    token >= vocab sets the error word and gives NaN
+ *   entropy [rows]   -sum p log p, in nats
+ *   rank [rows]      how many logits come before the token's, larger ones
+ *                    first and equal ones by index (0: the most likely); -1
+ *                    where the row has no token
+ *   top_ids, top_logprobs [rows][n_top]   the n_top (0..32) most likely
+ *                    tokens in that order
+ * Each output may be NULL; tokens may be NULL without logprob and rank. A
+ * logit of -inf has no probability; a row of nothing else (or with a NaN, or
+ * +inf) has NaN log probabilities and entropy, and is still ranked (NaN as
+ * -inf). Sums in fp32, in an order fixed by the shape: the same bits every
+ * time. Asynchronous on stream; no workspace. The reference computes none of
+ * these (its sampler keeps the probabilities, self/ml/gpu_sampler.hexa:89-140). */
+#define FORGE_LOGITS_F32  0
+#define FORGE_LOGITS_BF16 1
+#define FORGE_LOGPROBS_MAX_TOP 32
+int forge_token_logprobs(const void* logits, int dtype, int64_t ld, int rows, int vocab, const int32_t* tokens,
+                         int n_top, float* logprob, float* entropy, int32_t* rank, int32_t* top_ids,
+                         float* top_logprobs, void* stream);
+
 /* Causal (or full) flash-attention prefill on the tcgen05 tensor cores:
  * q, k, v, o [B][H][S][hd] bf16 device arrays (16-byte aligned), hd = 128 or 64,
  * S a multiple of 128; O = softmax(Q K^T / sqrt(hd) + mask) V with fp32
@@ -299,6 +323,27 @@ int forge_sample(const float* logits, int64_t ld, int batch, int vocab, double t
  * out) show in forge_ops_check(). */
 int forge_flash_prefill(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* o, int B, int H, int S,
                         int hd, int causal, void* stream);
+
+/* Causal prefill of packed prompts with grouped heads: n_seq sequences back
+ * to back, sequence s in rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device
+ * int32 [n_seq + 1], any lengths, zero among them) of q [total][ldq], k
+ * [total][ldk], v [total][ldv] (bf16; head h at h * hd, so the three can be
+ * parts of one projection's rows), query head h reading KV head h / (H / Hkv),
+ * hd 128 or 64:
+ *   o[i] = softmax(q[i] K^T / sqrt(hd)) V over the keys of i's sequence up to
+ *   i, to o [total][ldo] in bf16 (P rounded to bf16 for the product with V,
+ *   the sums in fp32);
+ *   lse[h][i] = log sum exp of that row's scores, fp32 [H][total], or NULL.
+ * Rows before cu_seqlens[0] and from cu_seqlens[n_seq] on are not written. A
+ * sequence whose bounds decrease or leave 0..total sets the error word
+ * (forge_ops_check) and is left out (rows that two of the others then share
+ * hold either's result). A NaN or infinity in k or v reaches its
+ * own sequence's rows only, there possibly rows up to 127 before it. Arrays
+ * 16-byte aligned, row lengths multiples of 8 elements; o must not overlap
+ * the inputs. Asynchronous on stream. */
+int forge_flash_prefill_varlen(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                               int64_t ldv, const int32_t* cu_seqlens, int n_seq, int total, int H, int Hkv, int hd,
+                               uint16_t* o, int64_t ldo, float* lse, void* stream);
 
 /* Weight preparation (device memory). */
 int forge_fill_normal_bf16(uint16_t* out, int64_t n, uint64_t seed, uint64_t offset, float std,

@@ -21,14 +21,16 @@
 //      registers: no chain of tensor-core sums is longer than 4.
 //
 // Work: the tiles of 64 keys of all (sequence, KV head, 8 query heads) form
-// one line, cut into one range per CTA, so a batch of very different lengths
-// is as even as one of equal ones. In a CTA each warp takes every fourth tile
-// with a ring of bulk copies and a softmax of its own; a sequence's end in the
-// range joins the four warps, and where a range ends inside a sequence the
-// last CTA to arrive joins the CTAs that shared it, in the order of the keys.
+// one line, every pair's tiles behind a few units for what a pair costs by
+// itself, cut into one range per CTA, so a batch of very different lengths is
+// as even as one of equal ones. In a CTA each warp takes every fourth tile
+// with a ring of bulk copies and a softmax of its own; a pair's end in the
+// range joins the four warps, and where a range ends inside a pair the last
+// CTA to arrive joins the CTAs that shared it, in the order of the keys.
 #include <cmath>
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "forge_internal.h"
 #include "../../include/forge_b200.h"
 #include "../../include/forge_kv4.h"
@@ -38,8 +40,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 64;          // keys per tile
 constexpr int kStages = 2;         // tiles a warp has in flight
-constexpr int kCtasPerSm = 3;
-constexpr int kMinTiles = kWarps;  // a range gives every warp a tile
+constexpr int kCtasPerSm = 2;
+constexpr int kPairUnits = 4;      // what a pair costs beside its tiles, in tiles
+constexpr int kMinUnits = kWarps + kPairUnits;  // a range of one pair gives every warp a tile
 constexpr int kHeads = 8;          // query heads that share a pass over the keys
 
 template <int HD>
@@ -47,9 +50,10 @@ struct Geo {
     static constexpr int kNG = HD / FORGE_KV4_GROUP;
     static constexpr int kCodes = kKeys * HD / 2, kScales = kKeys * kNG * 2;  // bytes of a tile, K or V
     static constexpr int kSlot = 2 * (kCodes + kScales);                      // K codes, V codes, K scales, V scales
-    static constexpr int kRedHeads = 256 / HD;                                // heads joined at a time
-    static constexpr int kOffRed = kWarps * kStages * kSlot;
-    static constexpr int kOffMl = kOffRed + kWarps * 256 * 4;                 // [warp][8] m, then l
+    static constexpr int kRow = HD + 4;                                       // floats of a head in the join (no bank twice)
+    static constexpr int kOffQ = kWarps * kStages * kSlot;                    // [4 groups][32 lanes] A operands
+    static constexpr int kOffRed = kOffQ + 4 * kNG * 512;                     // [warp][8][kRow] sums of the warps
+    static constexpr int kOffMl = kOffRed + kWarps * kHeads * kRow * 4;       // [warp][8] m, then l
     static constexpr int kOffBar = kOffMl + 2 * kWarps * kHeads * 4;
     static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
 };
@@ -67,25 +71,25 @@ struct Kv4Args {
     uint32_t* err;
 };
 
+// d = A B (+ c): m16n8k16, fp16 operands, fp32 sums.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-__device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // x as fp16 and what that leaves, two values at once
-__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    hi = h2bits(h);
-    lo = h2bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
+__device__ __forceinline__ void split_f16(F2 x, uint32_t& hi, uint32_t& lo) {
+    float r0, r1;  // hi - x
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x.y()), "f"(x.x()));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}"
+        : "=f"(r0), "=f"(r1) : "r"(hi), "f"(x.x()), "f"(x.y()));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(-r1), "f"(-r0));
 }
 // The codes in bits 0-3 (lo) or 4-7 (hi) of both halves, less 7 and times
 // 2^-9, as an fp16 pair (exact).
@@ -105,28 +109,33 @@ __device__ __forceinline__ int tiles_of(const Kv4Args& a, int b) {
     return (p >= a.cap || s < 0 || s >= a.c.n_seq) ? -1 : p / kKeys + 1;
 }
 
-// A place on the line of tiles: tile j of n of pair `pair` of sequence slot b.
+// A pair on the line: pair `pair` of sequence slot b, n tiles, units base ..
+// base + kPairUnits + n - 1.
 struct Place {
-    int b, pair, j, n;
-    __device__ void settle(const Kv4Args& a) {  // after j grew; the place is on the line
-        while (j >= n) {
-            j -= n;
-            if (++pair == a.ph) {
-                pair = 0;
-                do n = ++b < a.B ? max(0, tiles_of(a, b)) : 1 << 30;
-                while (n == 0);
-            }
+    int b, pair, n, base;
+    __device__ void next(const Kv4Args& a) {  // (behind the last pair: a place past every range)
+        base += kPairUnits + n;
+        if (++pair == a.ph) {
+            pair = 0;
+            do n = ++b < a.B ? max(0, tiles_of(a, b)) : 1 << 29;
+            while (n == 0);
         }
     }
+    // tiles of the pair inside units [start, end)
+    __device__ int lo(int start) const { return max(0, start - base - kPairUnits); }
+    __device__ int hi(int end) const { return min(n, end - base - kPairUnits); }
+    // first tile at or behind j that is warp w's
+    __device__ int mine(int j, int w) const { return j + ((w - j - pair) & (kWarps - 1)); }
 };
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Args a) {
     using X = Geo<HD>;
-    constexpr int NG = X::kNG;
+    constexpr int NG = X::kNG, U = kKeys / 8, KK = kKeys / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kStages * X::kSlot;
+    uint4* qs = reinterpret_cast<uint4*>(smem + X::kOffQ);
     float* red = reinterpret_cast<float*>(smem + X::kOffRed);
     float* sm_m = reinterpret_cast<float*>(smem + X::kOffMl);
     float* sm_l = sm_m + kWarps * kHeads;
@@ -139,10 +148,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
     }
 
     // ---- the line's length; sequences without tiles are answered here
-    long long total = 0;
+    int total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int b = b0 + lane;
-        int n = b < a.B ? tiles_of(a, b) : 0;
+        const int n = b < a.B ? tiles_of(a, b) : 0;
         if (warp == 0) {
             unsigned none = __ballot_sync(0xffffffffu, b < a.B && n <= 0 && b % (int)gridDim.x == (int)blockIdx.x);
             for (; none; none &= none - 1) {
@@ -153,105 +162,105 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
                 for (int i = lane; i < a.H * HD; i += 32) o[i] = bad ? NAN : 0.f;
             }
         }
-        n = max(n, 0);
-        total += __reduce_add_sync(0xffffffffu, n);
+        total += __reduce_add_sync(0xffffffffu, n > 0 ? n + kPairUnits : 0);
     }
     total *= a.ph;
-    const long long per = max((long long)kMinTiles, (total + gridDim.x - 1) / gridDim.x);
-    const long long start = (long long)blockIdx.x * per, end = min(total, start + per);
+    const int per = max(kMinUnits, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int start = (int)blockIdx.x * per, end = min(total, start + per);
     if (start >= end) return;
 
-    // ---- the place where this CTA's range starts
+    // ---- the pair in which this CTA's range starts
     Place at{0, 0, 0, 0};
-    long long base = 0;  // line index of the first tile of slot at.b
-    for (int b0 = 0;; b0 += 32) {
+    for (int b0 = 0;; b0 += 32) {  // at.base: first unit of slot b0
         const int b = b0 + lane;
-        const int n = b < a.B ? max(0, tiles_of(a, b)) : 0;
-        int inc = n;
+        const int n = b < a.B ? max(0, tiles_of(a, b)) : 0, un = n ? n + kPairUnits : 0;
+        int inc = un;
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += u;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, base + (long long)inc * a.ph > start);
+        const unsigned past = __ballot_sync(0xffffffffu, at.base + inc * a.ph > start);
         if (past) {
             const int w = __ffs(past) - 1;
             at.n = __shfl_sync(0xffffffffu, n, w);
-            base += (long long)(__shfl_sync(0xffffffffu, inc, w) - at.n) * a.ph;
+            const int units = at.n + kPairUnits;
+            at.base += (__shfl_sync(0xffffffffu, inc, w) - units) * a.ph;
             at.b = b0 + w;
-            at.pair = (int)((start - base) / at.n);
-            at.j = (int)(start - base - (long long)at.pair * at.n);
+            at.pair = (start - at.base) / units;
+            at.base += at.pair * units;
             break;
         }
-        base += (long long)__shfl_sync(0xffffffffu, inc, 31) * a.ph;
+        at.base += __shfl_sync(0xffffffffu, inc, 31) * a.ph;
     }
-    __syncwarp();
 
-    // ---- copies of this warp's tiles start + warp, + 4, ...
+    // ---- copies of this warp's tiles: lane 4 i + k copies array k (K codes, V codes, K scales, V scales) of the
+    // tile's i-th page
+    const int arr = lane & 3;
+    const int unit = arr < 2 ? HD / 2 : NG * 2;  // bytes a row
+    const int slot_off = arr == 0 ? 0 : arr == 1 ? X::kCodes : 2 * X::kCodes + (arr - 2) * X::kScales;
+    const uint8_t* array = arr == 0 ? a.c.k : arr == 1 ? a.c.v : (const uint8_t*)(arr == 2 ? a.c.ks : a.c.vs);
     Place in = at;
-    in.j += warp;
-    long long f_in = start + warp;
-    int n_in = 0;
-    uint32_t poison = 0;  // slots whose tile names a page outside the pool
-    if (f_in < end) in.settle(a);
+    int in_j = in.mine(in.lo(start), warp), n_in = 0;
+    uint32_t poison = 0;      // slots whose tile names a page outside the pool
+    int in_rows = 0;          // rows of the pair's sequence, in eights
+    int64_t in_row0 = 0;      // contiguous: its first row in the arrays; paged: KV head
+    const int32_t* in_table = nullptr;
+    bool entered = false;
     auto issue = [&]() {
-        if (f_in >= end) return;
-        const int s = n_in % kStages;
-        const int L = a.pos[in.b] + 1, sq = a.seq ? a.seq[in.b] : in.b, kvh = in.pair / a.nhb;
-        const int key0 = in.j * kKeys;
-        const int rows = min(kKeys, (L - key0 + 7) & ~7);
-        uint8_t* dst = ring + s * X::kSlot;
+        while (in_j >= in.hi(end)) {
+            if (in.base >= end) return;
+            in.next(a);
+            in_j = in.mine(0, warp);
+            entered = false;
+        }
+        if (!entered) {
+            const int sq = a.seq ? a.seq[in.b] : in.b, kvh = in.pair / a.nhb;
+            in_rows = (a.pos[in.b] + 8) & ~7;
+            in_row0 = a.c.table ? kvh : ((int64_t)sq * a.c.n_kv_head + kvh) * a.c.lmax;
+            in_table = a.c.table ? a.c.table + (int64_t)sq * a.c.max_pages : nullptr;
+            entered = true;
+        }
+        const int s = n_in % kStages, key0 = in_j * kKeys;
+        const int rows = min(kKeys, in_rows - key0);
+        uint8_t* dst = ring + s * X::kSlot + slot_off;
         if (lane == 0) mbar_arrive_expect_tx(&full[s], rows * (HD + 4 * NG));
         __syncwarp();
-        // lane 4i + k copies array k (K codes, V codes, K scales, V scales) of segment i
-        const int seg = lane >> 2, arr = lane & 3;
-        int r0 = 0, r1 = rows;
-        int64_t row = 0;
-        bool bad = false;
-        if (!a.c.table) {
-            if (seg) r1 = 0;
-            row = ((int64_t)sq * a.c.n_kv_head + kvh) * a.c.lmax + key0;
+        if (!in_table) {
+            if (lane < 4) bulk_g2s_stream(dst, array + (in_row0 + key0) * unit, rows * unit, &full[s], l2_evict_first());
         } else {
-            const int pt = a.c.page_tokens, pg0 = key0 / pt;
-            r0 = max(0, (pg0 + seg) * pt - key0);
-            r1 = min(rows, (pg0 + seg + 1) * pt - key0);
+            const int pt = a.c.page_tokens, pg0 = key0 / pt + (lane >> 2);
+            const int r0 = max(0, pg0 * pt - key0), r1 = min(rows, (pg0 + 1) * pt - key0);
+            bool bad = false;
             if (r0 < r1) {
-                int pg = a.c.table[(int64_t)sq * a.c.max_pages + pg0 + seg];
+                int pg = in_table[pg0];
                 bad = (unsigned)pg >= (unsigned)a.c.num_pages;
                 if (bad) {
                     atomicOr(a.err, FORGE_DEVERR_BAD_INDEX);
                     pg = 0;
                 }
-                row = ((int64_t)pg * a.c.n_kv_head + kvh) * pt + (key0 + r0) % pt;
+                const int64_t row = ((int64_t)pg * a.c.n_kv_head + in_row0) * pt + (key0 + r0 - pg0 * pt);
+                bulk_g2s_stream(dst + r0 * unit, array + row * unit, (r1 - r0) * unit, &full[s], l2_evict_first());
             }
+            poison &= ~(1u << s);
+            if (__any_sync(0xffffffffu, bad)) poison |= 1u << s;
         }
-        if (r0 < r1) {
-            const int unit = arr < 2 ? HD / 2 : NG * 2;  // bytes a row
-            const uint8_t* src = arr == 0 ? a.c.k : arr == 1 ? a.c.v : (const uint8_t*)(arr == 2 ? a.c.ks : a.c.vs);
-            const int off = arr == 0 ? 0 : arr == 1 ? X::kCodes : 2 * X::kCodes + (arr - 2) * X::kScales;
-            bulk_g2s_stream(dst + off + r0 * unit, src + row * unit, (r1 - r0) * unit, &full[s], l2_evict_first());
-        }
-        poison &= ~(1u << s);
-        if (__any_sync(0xffffffffu, bad)) poison |= 1u << s;
-        f_in += kWarps;
+        in_j += kWarps;
         ++n_in;
-        in.j += kWarps;
-        if (f_in < end) in.settle(a);
     };
     for (int s = 0; s < kStages; ++s) issue();
 
     int n_out = 0;
     bool dead = false;  // a wait ran out: nothing more is read
-    for (long long f = start; f < end;) {
-        // ---- one sequence's pair: tiles [f, f1) of the line
-        const long long pair0 = f - at.j, pair1 = pair0 + at.n, f1 = min(end, pair1);
+    for (; at.base < end; at.next(a)) {
+        // ---- one pair: tiles [j0, j1)
+        const int j0 = at.lo(start), j1 = at.hi(end);
+        if (j0 >= j1) continue;
         const int kvh = at.pair / a.nhb, h0 = (at.pair % a.nhb) * kHeads, nh = min(kHeads, a.G - h0);
-        const int L = a.pos[at.b] + 1;
         const size_t qrow = (size_t)at.b * a.H + kvh * a.G + h0;
 
-        // q as A operands: head g, dims 64 gr + 16 t + 8 w + {0..7}; fp16 pairs (d, d + 4) and (d + 1, d + 5)
+        // q as A operands: head g, dims 64 i + 16 t + 8 w + {0..7}, fp16 pairs (d, d + 4) and (d + 1, d + 5)
         // (in shared memory, one quarter from each warp: registers are short while the codes of V are unpacked)
         float fac;
-        uint4* qs = reinterpret_cast<uint4*>(red);  // [4 NG][32 lanes]
         {
             float4 v[NG][4];
             float mx = 0.f;
@@ -267,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             // 2^e <= mx < 2^(e + 1); q 2^(14 - e) fits fp16
             const int e = max(-110, min(120, (int)(__float_as_uint(mx) >> 23) - 127));
-            const float up = pow2i(14 - e);
+            const F2 up(pow2i(14 - e), pow2i(14 - e));
             fac = a.scale_log2 * 0x1p-5f * pow2i(e);  // 2^9 of the codes, 2^(e - 14) of q
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
@@ -275,22 +284,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
                 const float4 lo4 = warp & 2 ? v[i][2] : v[i][0], hi4 = warp & 2 ? v[i][3] : v[i][1];
                 const bool k = warp & 1;
                 uint4 r;
-                split_f16((k ? lo4.z : lo4.x) * up, (k ? hi4.z : hi4.x) * up, r.x, r.y);
-                split_f16((k ? lo4.w : lo4.y) * up, (k ? hi4.w : hi4.y) * up, r.z, r.w);
+                split_f16(F2(k ? lo4.z : lo4.x, k ? hi4.z : hi4.x) * up, r.x, r.y);
+                split_f16(F2(k ? lo4.w : lo4.y, k ? hi4.w : hi4.y) * up, r.z, r.w);
                 qs[(4 * i + warp) * 32 + lane] = r;
             }
         }
         __syncthreads();
 
-        float m = -INFINITY, l = 0.f;
-        float o[NG][8][2];  // [group][nibble][column pair]: dims 64 i + 16 t + n and + 8, times 2^(-9 + 14 - e_run)
-        int e_run = -100;
+        // p_j = 2^(x_j - mref), mref = max x - 14 + e, e following the largest V scale: weights p_j sv_j stay below
+        // 2^14; l and o (times 2^9) are sums of those p
+        float m = -INFINITY, mref = -INFINITY;
+        F2 l(0.f, 0.f), o[NG][8];  // o[group][nibble]: dims 64 i + 16 t + n and + 8
+        int e_run = -88;
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) o[i][n][0] = o[i][n][1] = 0.f;
+            for (int n = 0; n < 8; ++n) o[i][n] = F2(0.f, 0.f);
 
-        for (long long ft = f + ((warp - (int)(f - start)) & (kWarps - 1)); ft < f1; ft += kWarps) {
+#pragma unroll 1
+        for (int j = at.mine(j0, warp); j < j1; j += kWarps) {
             if (dead) break;
             const int s = n_out % kStages;
             if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (n_out / kStages) & 1, a.err))) {
@@ -301,256 +313,223 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             const uint8_t* kc = ring + s * X::kSlot;
             const uint8_t* vc = kc + X::kCodes;
             const uint8_t* ks = vc + X::kCodes;
-            const uint8_t* vs = ks + X::kScales;
-            const int left = L - (int)(ft - pair0) * kKeys;  // valid keys of the tile (may be more than 64)
+            uint8_t* vs = const_cast<uint8_t*>(ks) + X::kScales;
+            const int left = j + 1 < at.n ? kKeys : a.pos[at.b] + 1 - j * kKeys;  // keys of the tile
 
-            // ---- scores of keys 8 u + t and 8 u + 4 + t, head g (log2 units)
-            uint32_t qa[NG][4][4];
+            // ---- scores of keys 8 u + t and 8 u + 4 + t, head g, over fac
+            F2 x[U];
 #pragma unroll
-            for (int i = 0; i < 4 * NG; ++i) {
-                const uint4 r = qs[i * 32 + lane];
-                qa[i / 4][i % 4][0] = r.x; qa[i / 4][i % 4][1] = r.y; qa[i / 4][i % 4][2] = r.z; qa[i / 4][i % 4][3] = r.w;
-            }
-            float x[8][2];
-            float mx = -INFINITY;
+            for (int i = 0; i < NG; ++i) {
+                uint32_t qa[4][4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const uint8_t* row = kc + (8 * u + (g >> 1) + 4 * (g & 1)) * (HD / 2) + t * 8;
-                float x0 = 0.f, x1 = 0.f;
-                uint32_t s0, s1;
-                if (NG == 2) {
-                    s0 = *reinterpret_cast<const uint32_t*>(ks + (8 * u + t) * 4);
-                    s1 = *reinterpret_cast<const uint32_t*>(ks + (8 * u + 4 + t) * 4);
-                } else {
-                    s0 = *reinterpret_cast<const uint16_t*>(ks + (8 * u + t) * 2);
-                    s1 = *reinterpret_cast<const uint16_t*>(ks + (8 * u + 4 + t) * 2);
+                for (int k = 0; k < 4; ++k) {
+                    const uint4 r = qs[(4 * i + k) * 32 + lane];
+                    qa[k][0] = r.x; qa[k][1] = r.y; qa[k][2] = r.z; qa[k][3] = r.w;
                 }
 #pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * i);
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(c, qa[i][0], code_lo(w.x), code_hi(w.x));
-                    mma_f16(c, qa[i][1], code_lo(w.x >> 8), code_hi(w.x >> 8));
-                    mma_f16(c, qa[i][2], code_lo(w.y), code_hi(w.y));
-                    mma_f16(c, qa[i][3], code_lo(w.y >> 8), code_hi(w.y >> 8));
-                    x0 = fmaf(c[0] + c[2], i ? bf16_hi_f32(s0) : bf16_lo_f32(s0), x0);
-                    x1 = fmaf(c[1] + c[3], i ? bf16_hi_f32(s1) : bf16_lo_f32(s1), x1);
+                for (int u = 0; u < U; ++u) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(kc + (8 * u + (g >> 1) + 4 * (g & 1)) * (HD / 2) + 32 * i + t * 8);
+                    const uint16_t s0 = *reinterpret_cast<const uint16_t*>(ks + ((8 * u + t) * NG + i) * 2);
+                    const uint16_t s1 = *reinterpret_cast<const uint16_t*>(ks + ((8 * u + 4 + t) * NG + i) * 2);
+                    float c[4];
+                    mma_f16_first(c, qa[0], code_lo(w.x), code_hi(w.x));
+                    mma_f16(c, qa[1], code_lo(w.x >> 8), code_hi(w.x >> 8));
+                    mma_f16(c, qa[2], code_lo(w.y), code_hi(w.y));
+                    mma_f16(c, qa[3], code_lo(w.y >> 8), code_hi(w.y >> 8));
+                    const F2 sum = F2(c[0], c[1]) + F2(c[2], c[3]), sc(bf16_bits_to_f32(s0), bf16_bits_to_f32(s1));
+                    x[u] = i ? fma2(sum, sc, x[u]) : sum * sc;
                 }
-                x[u][0] = x0 * fac;
-                x[u][1] = x1 * fac;
             }
-            // ---- scales of V; keys behind the last one count for nothing
-            uint32_t sv[8][2];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    sv[u][k] = NG == 2 ? *reinterpret_cast<const uint32_t*>(vs + (8 * u + 4 * k + t) * 4)
-                                       : *reinterpret_cast<const uint16_t*>(vs + (8 * u + 4 * k + t) * 2);
+            // ---- the tile's largest score and V scale; keys behind the last one count for nothing
             if (left < kKeys) {
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < U; ++u)
+                    x[u] = F2(8 * u + t < left ? x[u].x() : -INFINITY, 8 * u + 4 + t < left ? x[u].y() : -INFINITY);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (8 * u + 4 * k + t >= left) {
-                            x[u][k] = -INFINITY;
-                            sv[u][k] = 0;
-                        }
+                for (int k = 0; k < kKeys * NG; k += 32)
+                    if (k + lane >= left * NG) reinterpret_cast<uint16_t*>(vs)[k + lane] = 0;
+                __syncwarp();
             }
-            __nv_bfloat162 smx = __floats2bfloat162_rn(0.f, 0.f);
+            uint32_t smax = 0;  // bf16 bits, two at a time
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+            for (int k = 0; k < kKeys * NG / 2; k += 32)
+                if (k + lane < kKeys * NG / 2) smax = __vmaxu2(smax, reinterpret_cast<const uint32_t*>(vs)[k + lane] & 0x7FFF7FFFu);
+            smax = __reduce_max_sync(0xffffffffu, max(smax & 0xffffu, smax >> 16));
+            float mx = fmaxf(x[0].x(), x[0].y());
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    mx = fmaxf(mx, x[u][k]);
-                    smx = __hmax2(smx, *reinterpret_cast<const __nv_bfloat162*>(&sv[u][k]));
-                }
+            for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            float sm = fmaxf(__low2float(smx), __high2float(smx));
-            sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, 1));
-            sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, 2));
-            const float m_new = fmaxf(m, mx);
-            float alpha = ex2(m - m_new);  // 0 at the first tile
-            if (m_new == -INFINITY) alpha = 1.f;
-            m = m_new;
-            const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-            // weights p sv 2^(14 - e) stay below 2^15; e follows the largest scale (the same in all lanes)
-            const int e = max(e_run, min(129, (int)(__float_as_uint(sm) >> 23) - 126));
-            const float up = pow2i(14 - e);
-            const float alpha_o = e_run - e < -126 ? 0.f : alpha * pow2i(e_run - e);
-            e_run = e;
-            float ls = 0.f;
+            m = fmaxf(m, mx * fac);
+            e_run = max(e_run, min(129, (int)(smax >> 7) - 126));  // the same in all lanes
+            const float m_new = m - (float)(14 - e_run);
+            const float alpha = mref == -INFINITY ? 0.f : ex2(mref - m_new);
+            mref = m_new;
+            const float nref = m_new == -INFINITY ? 0.f : -m_new;
+            F2 ls;
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float p = ex2(x[u][k] - m_ref);
-                    ls += p;
-                    x[u][k] = p * up;
-                }
-            l = fmaf(l, alpha, ls);
+            for (int u = 0; u < U; ++u) {
+                const F2 y = fma2(x[u], F2(fac, fac), F2(nref, nref));
+                x[u] = F2(ex2(y.x()), ex2(y.y()));
+                ls = u ? ls + x[u] : x[u];
+            }
+            l = fma2(l, F2(alpha, alpha), ls);
 
             // ---- O += P V, group by group
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 float c[8][4];
 #pragma unroll
-                for (int n = 0; n < 8; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
+                for (int kk = 0; kk < KK; ++kk) {
                     uint32_t pa[4];
-                    float w[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t s2 = sv[2 * kk + (j >> 1)][j & 1];
-                        w[j] = x[2 * kk + (j >> 1)][j & 1] * (i ? bf16_hi_f32(s2) : bf16_lo_f32(s2));
+                    for (int k = 0; k < 2; ++k) {
+                        const int key = 16 * kk + 8 * k + t;
+                        const uint16_t s0 = *reinterpret_cast<const uint16_t*>(vs + (key * NG + i) * 2);
+                        const uint16_t s1 = *reinterpret_cast<const uint16_t*>(vs + ((key + 4) * NG + i) * 2);
+                        split_f16(x[2 * kk + k] * F2(bf16_bits_to_f32(s0), bf16_bits_to_f32(s1)), pa[2 * k], pa[2 * k + 1]);
                     }
-                    split_f16(w[0], w[1], pa[0], pa[1]);
-                    split_f16(w[2], w[3], pa[2], pa[3]);
                     uint32_t r[4];  // word g of group i of keys 16 kk + t + {0, 4, 8, 12}
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        r[j] = *reinterpret_cast<const uint32_t*>(vc + (16 * kk + 4 * j + t) * (HD / 2) + 32 * i + 4 * g);
+                    for (int k = 0; k < 4; ++k)
+                        r[k] = *reinterpret_cast<const uint32_t*>(vc + (16 * kk + 4 * k + t) * (HD / 2) + 32 * i + 4 * g);
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        // nibbles 4 hf .. 4 hf + 3 of two keys side by side
-                        const uint32_t p0 = __byte_perm(r[0], r[1], hf ? 0x7632 : 0x5410);
-                        const uint32_t p1 = __byte_perm(r[2], r[3], hf ? 0x7632 : 0x5410);
-                        mma_f16(c[4 * hf + 0], pa, code_lo(p0), code_lo(p1));
-                        mma_f16(c[4 * hf + 1], pa, code_hi(p0), code_hi(p1));
-                        mma_f16(c[4 * hf + 2], pa, code_lo(p0 >> 8), code_lo(p1 >> 8));
-                        mma_f16(c[4 * hf + 3], pa, code_hi(p0 >> 8), code_hi(p1 >> 8));
+                    for (int k = 0; k < 4; ++k) {
+                        // byte k (nibbles 2 k and 2 k + 1) of two keys, one in either half
+                        const uint32_t p0 = __byte_perm(r[0], r[1], 0x4400 + 0x1111 * k);
+                        const uint32_t p1 = __byte_perm(r[2], r[3], 0x4400 + 0x1111 * k);
+                        if (kk == 0) {
+                            mma_f16_first(c[2 * k], pa, code_lo(p0), code_lo(p1));
+                            mma_f16_first(c[2 * k + 1], pa, code_hi(p0), code_hi(p1));
+                        } else {
+                            mma_f16(c[2 * k], pa, code_lo(p0), code_lo(p1));
+                            mma_f16(c[2 * k + 1], pa, code_hi(p0), code_hi(p1));
+                        }
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    o[i][n][0] = fmaf(o[i][n][0], alpha_o, c[n][0] + c[n][2]);
-                    o[i][n][1] = fmaf(o[i][n][1], alpha_o, c[n][1] + c[n][3]);
-                }
+                for (int n = 0; n < 8; ++n)
+                    o[i][n] = fma2(o[i][n], F2(alpha, alpha), F2(c[n][0], c[n][1]) + F2(c[n][2], c[n][3]));
             }
-            if (poison >> s & 1) l = NAN;
+            if (poison >> s & 1) l = F2(NAN, NAN);
             ++n_out;
             __syncwarp();
             issue();
         }
-        if (dead) l = NAN;
+        if (dead) l = F2(NAN, NAN);
 
-        // ---- join the warps: O / l of the CTA's keys, with their (m, l)
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        // ---- join the warps: their sums with their (mref, l)
+        float lw = l.x() + l.y();
+        lw += __shfl_xor_sync(0xffffffffu, lw, 1);
+        lw += __shfl_xor_sync(0xffffffffu, lw, 2);
         if (t == 0) {
-            sm_m[warp * kHeads + g] = m;
-            sm_l[warp * kHeads + g] = l;
+            sm_m[warp * kHeads + g] = mref;
+            sm_l[warp * kHeads + g] = lw;
+        }
+        if (g < nh) {
+            float* dst = red + (warp * kHeads + g) * X::kRow + 16 * t;
+#pragma unroll
+            for (int i = 0; i < NG; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int n = 0; n < 8; n += 4) {
+                        float4 v;
+                        v.x = k ? o[i][n].y() : o[i][n].x();
+                        v.y = k ? o[i][n + 1].y() : o[i][n + 1].x();
+                        v.z = k ? o[i][n + 2].y() : o[i][n + 2].x();
+                        v.w = k ? o[i][n + 3].y() : o[i][n + 3].x();
+                        *reinterpret_cast<float4*>(dst + 64 * i + 8 * k + n) = v;
+                    }
         }
         __syncthreads();
-        float mj = -INFINITY, lj = 0.f;
+        const int unit0 = at.base + kPairUnits, cfirst = unit0 / per, clast = (unit0 + at.n - 1) / per;
+        float* part = a.partial + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == cfirst)) * kHeads * (HD + 2);
+        for (int idx = threadIdx.x; idx < nh * (HD / 4); idx += kThreads) {
+            const int h = idx / (HD / 4), d = idx % (HD / 4) * 4;
+            float mj = -INFINITY, lj = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mj = fmaxf(mj, sm_m[w * kHeads + g]);
+            for (int w = 0; w < kWarps; ++w) mj = fmaxf(mj, sm_m[w * kHeads + h]);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float mw = sm_m[w * kHeads + g];
-            lj = fmaf(sm_l[w * kHeads + g], mw == -INFINITY ? 0.f : ex2(mw - mj), lj);
-            if (isnan(sm_l[w * kHeads + g])) lj = NAN;
-        }
-        // o 2^(e_run - 5) ex2(m - mj) / lj
-        const float fo = (m == -INFINITY ? 0.f : ex2(m - mj)) / lj * 0x1p15f;
-        const float up0 = pow2i(e_run - 20);
-        const bool whole = f == pair0 && f1 == pair1;  // no other CTA shares the pair
-        const long long cfirst = pair0 / per, clast = (pair1 - 1) / per;
-        float* part = a.partial + ((size_t)blockIdx.x * 2 + (blockIdx.x == cfirst)) * kHeads * (HD + 2);
-        constexpr int RH = X::kRedHeads;
-        for (int hr = 0; hr < nh; hr += RH) {
-            if (g >= hr && g < hr + RH) {
-                float* dst = red + (warp * RH + g - hr) * HD;
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-                            dst[64 * i + 16 * t + 8 * k + n] = o[i][n][k] * fo * up0;
+            for (int w = 0; w < kWarps; ++w) {
+                const float mw = sm_m[w * kHeads + h], lv = sm_l[w * kHeads + h];
+                const float f = mw == -INFINITY ? 0.f : ex2(mw - mj);
+                lj = isnan(lv) ? lv : fmaf(lv, f, lj);
+                const float4 r = *reinterpret_cast<const float4*>(red + (w * kHeads + h) * X::kRow + d);
+                v.x = fmaf(r.x, f, v.x); v.y = fmaf(r.y, f, v.y); v.z = fmaf(r.z, f, v.z); v.w = fmaf(r.w, f, v.w);
             }
-            __syncthreads();
-            for (int idx = threadIdx.x; idx < RH * HD; idx += kThreads) {
-                const int h = hr + idx / HD, d = idx % HD;
-                if (h < nh) {
-                    float v = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) v += red[w * RH * HD + idx];
-                    if (whole) a.out[(qrow + h) * HD + d] = v;
-                    else part[h * (HD + 2) + d] = v;
+            const float il = 512.f / lj;
+            v.x *= il; v.y *= il; v.z *= il; v.w *= il;
+            if (cfirst == clast) {
+                *reinterpret_cast<float4*>(a.out + (qrow + h) * HD + d) = v;
+            } else {
+                float2* dst = reinterpret_cast<float2*>(part + h * (HD + 2) + d);
+                dst[0] = make_float2(v.x, v.y);
+                dst[1] = make_float2(v.z, v.w);
+                if (d == 0) {
+                    part[h * (HD + 2) + HD] = mj;
+                    part[h * (HD + 2) + HD + 1] = lj;
                 }
             }
-            __syncthreads();
         }
-        if (!whole) {
-            if (warp == 0 && t == 0 && g < nh) {
-                part[g * (HD + 2) + HD] = mj;
-                part[g * (HD + 2) + HD + 1] = lj;
-            }
-            // the last of the pair's CTAs joins them: the block barrier orders
-            // the partial's stores before thread 0's release
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint32_t old;
-                const uint32_t top = (uint32_t)(clast - cfirst);  // the counter returns to 0 after the last
-                asm volatile("fence.acq_rel.gpu;" ::: "memory");
-                asm volatile("atom.inc.acq_rel.gpu.global.u32 %0, [%1], %2;"
-                             : "=r"(old) : "l"(a.counters + (size_t)at.b * a.ph + at.pair), "r"(top) : "memory");
-                s_last = old == top;
-            }
-            __syncthreads();
-            if (s_last) {
-                const int nc = (int)(clast - cfirst) + 1;
-                for (int h = warp; h < nh; h += kWarps) {
-                    // slot of contribution c: the pair starts in the first CTA's range and before every other's
-                    auto slot = [&](int c) {
-                        return a.partial + (((size_t)cfirst + c) * 2 + (c == 0)) * kHeads * (HD + 2) + h * (HD + 2);
-                    };
-                    float mm = -INFINITY;
-                    for (int c = lane; c < nc; c += 32) mm = fmaxf(mm, __ldcg(slot(c) + HD));
-                    for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-                    constexpr int E = HD / 32;
-                    float acc[E] = {}, sum = 0.f;
-                    for (int c0 = 0; c0 < nc; c0 += 32) {
-                        float wl = 0.f;
-                        if (c0 + lane < nc) {
-                            const float mc = __ldcg(slot(c0 + lane) + HD), lc = __ldcg(slot(c0 + lane) + HD + 1);
-                            wl = mc == -INFINITY && !isnan(lc) ? 0.f : lc * ex2(mc - mm);
-                        }
-                        const int cn = min(32, nc - c0);
-                        for (int c = 0; c < cn; c += 8) {
-                            float2 v[8][E / 2];
+        if (cfirst == clast) continue;
+        // ---- the last of the pair's CTAs joins them: the block barrier orders the partial's stores before thread 0's
+        // release
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t old;
+            const uint32_t top = clast - cfirst;  // the counter returns to 0 after the last
+            asm volatile("fence.acq_rel.gpu;" ::: "memory");
+            asm volatile("atom.inc.acq_rel.gpu.global.u32 %0, [%1], %2;"
+                         : "=r"(old) : "l"(a.counters + (size_t)at.b * a.ph + at.pair), "r"(top) : "memory");
+            s_last = old == top;
+        }
+        __syncthreads();
+        if (!s_last) continue;
+        const int nc = clast - cfirst + 1;
+        for (int h = warp; h < nh; h += kWarps) {
+            // contribution c: the pair starts in the first CTA's range and before every other's
+            auto slot = [&](int c) {
+                return a.partial + ((size_t)(cfirst + c) * 2 + (c == 0)) * kHeads * (HD + 2) + h * (HD + 2);
+            };
+            float mm = -INFINITY;
+            for (int c = lane; c < nc; c += 32) mm = fmaxf(mm, __ldcg(slot(c) + HD));
+            for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+            constexpr int E = HD / 32;
+            float acc[E] = {}, sum = 0.f;
+            for (int c0 = 0; c0 < nc; c0 += 32) {
+                float wl = 0.f;
+                if (c0 + lane < nc) {
+                    const float mc = __ldcg(slot(c0 + lane) + HD), lc = __ldcg(slot(c0 + lane) + HD + 1);
+                    wl = mc == -INFINITY && !isnan(lc) ? 0.f : lc * ex2(mc - mm);
+                }
+                const int cn = min(32, nc - c0);
+                for (int c = 0; c < cn; c += 8) {
+                    float2 v[8][E / 2];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
+                    for (int k = 0; k < 8; ++k)
 #pragma unroll
-                                for (int k = 0; k < E / 2; ++k)
-                                    if (c + j < cn) v[j][k] = __ldcg(reinterpret_cast<const float2*>(slot(c0 + c + j)) + 32 * k + lane);
+                        for (int e = 0; e < E / 2; ++e)
+                            if (c + k < cn) v[k][e] = __ldcg(reinterpret_cast<const float2*>(slot(c0 + c + k)) + 32 * e + lane);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float w = __shfl_sync(0xffffffffu, wl, (c + j) & 31);
-                                if (c + j < cn) {
-                                    sum += w;
+                    for (int k = 0; k < 8; ++k) {
+                        const float w = __shfl_sync(0xffffffffu, wl, (c + k) & 31);
+                        if (c + k < cn) {
+                            sum += w;
 #pragma unroll
-                                    for (int k = 0; k < E / 2; ++k) {
-                                        acc[2 * k] = w == 0.f ? acc[2 * k] : fmaf(w, v[j][k].x, acc[2 * k]);
-                                        acc[2 * k + 1] = w == 0.f ? acc[2 * k + 1] : fmaf(w, v[j][k].y, acc[2 * k + 1]);
-                                    }
-                                }
+                            for (int e = 0; e < E / 2; ++e) {
+                                acc[2 * e] = w == 0.f ? acc[2 * e] : fmaf(w, v[k][e].x, acc[2 * e]);
+                                acc[2 * e + 1] = w == 0.f ? acc[2 * e + 1] : fmaf(w, v[k][e].y, acc[2 * e + 1]);
                             }
                         }
                     }
-#pragma unroll
-                    for (int k = 0; k < E / 2; ++k)
-                        reinterpret_cast<float2*>(a.out + (qrow + h) * HD)[32 * k + lane] =
-                            make_float2(acc[2 * k] / sum, acc[2 * k + 1] / sum);
                 }
             }
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e)
+                reinterpret_cast<float2*>(a.out + (qrow + h) * HD)[32 * e + lane] = make_float2(acc[2 * e] / sum, acc[2 * e + 1] / sum);
         }
-        f = f1;
-        at.j = (int)(f1 - pair0);
-        if (f < end) at.settle(a);
     }
 }
 
@@ -587,22 +566,25 @@ extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* 
     if (!q || !pos || !out || !workspace || B <= 0 || B > 65535 || H <= 0 || H % cache->n_kv_head ||
         (!seq && B > cache->n_seq) || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15))
         return forge_fail(FORGE_INVALID_ARGS, "forge_flash_decode_kv4: bad args (arrays 16-byte aligned, H a multiple of the KV heads)");
+    const int hd = cache->head_dim, cap = cache->table ? cache->max_pages * cache->page_tokens : cache->lmax;
+    const int64_t units = (int64_t)B * cache->n_kv_head * ((H / cache->n_kv_head + kHeads - 1) / kHeads) * ((cap + kKeys - 1) / kKeys + kPairUnits);
+    if (units > (1ll << 30))
+        return forge_fail(FORGE_INVALID_ARGS, "forge_flash_decode_kv4: B x KV heads x rows of a sequence is too large (%lld tiles of 64 keys)", (long long)units);
     uint32_t* err = forge_ops_err_word();
     if (!err) return forge_fail(-1, "forge_flash_decode_kv4: no device");
     if (configure()) return -1;
-    const int hd = cache->head_dim;
     Kv4Args a{};
     a.c = *cache; a.q = q; a.seq = seq; a.pos = pos; a.B = B; a.H = H;
     a.G = H / cache->n_kv_head;
     a.nhb = (a.G + kHeads - 1) / kHeads;
     a.ph = cache->n_kv_head * a.nhb;
-    a.cap = cache->table ? cache->max_pages * cache->page_tokens : cache->lmax;
+    a.cap = cap;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.out = out; a.err = err;
     a.counters = (uint32_t*)workspace;
     a.partial = (float*)((char*)workspace + counter_bytes(B, H, cache->n_kv_head));
     // no more CTAs than the longest sequences could feed
-    const int64_t most = ((int64_t)B * a.ph * ((a.cap + kKeys - 1) / kKeys) + kMinTiles - 1) / kMinTiles;
+    const int64_t most = (units + kMinUnits - 1) / kMinUnits;
     const int grid = (int)(most < kMaxCtas ? most : kMaxCtas);
     if (hd == 128) k_kv4_decode<128><<<grid, kThreads, Geo<128>::kSmem, (cudaStream_t)stream>>>(a);
     else k_kv4_decode<64><<<grid, kThreads, Geo<64>::kSmem, (cudaStream_t)stream>>>(a);

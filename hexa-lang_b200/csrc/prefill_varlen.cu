@@ -8,24 +8,28 @@
 // A work item is two tiles of 128 query rows that share every K/V block: two
 // query heads of one KV head where the group is even (the tiles then have the
 // same blocks, and a short prompt fills both), else two consecutive tiles of
-// one head. CTAs are persistent, one per SM; items are ordered by the number
-// of their key blocks, longest first, and dealt out back and forth, so each
-// CTA gets about the same work whatever the lengths. The order needs no table:
-// item k's depth p is where the number of tiles at depth p or more, a sum over
-// the sequences, passes k (a few warp-wide sums by a warp of its own, one item
-// ahead of the others).
+// one head. CTAs are persistent, one per SM. Items are dealt out longest
+// first: for every depth (position of the tile in its sequence) from the
+// deepest, its items raise the CTAs' loads to a common level. Every CTA works
+// this out for itself, in a warp of its own that runs ahead of the others, so
+// that any mix of lengths is even without a table, a counter or a second
+// launch (dealing the sorted items out back and forth instead took 1.4 times
+// as long for 8 prompts of 1 to 1024 tokens).
 //
 //   warps 0-3 / 4-7    softmax of tile A / B, one thread per query row
-//   warp 8             TMA: Q of both tiles, K and V through a 4-slot ring
+//   warp 8             TMA: Q of both tiles, K and V through a 5-slot ring
 //   warp 9 (one lane)  tensor-core issue, tiles alternating
 //   warp 10            items
 //
-// S = Q K^T (128 x 128 x hd) goes to TMEM; its thread takes the whole row into
-// registers (setmaxnreg moves registers from the other warps), so TMEM is read
-// once and P = 2^(S c - m) can overwrite S as bf16 pairs, the A operand of
-// O += P V. P is handed over in two halves: the product of the first 64 keys
-// runs while the second half's exponentials do. m is raised only when a score
-// exceeds it by more than 2^8, so O in TMEM is rarely rescaled.
+// Keys are taken 64 at a time (half a block): S = Q K^T (128 x 64 x hd) goes to
+// one of two TMEM buffers of its tile; its thread takes the row into
+// registers and writes P = 2^(S c - m) over it as bf16 pairs, the A operand of
+// O += P V. With two buffers the tensor cores run S of the next half block
+// while the exponentials of this one run: a tile's softmax never waits for
+// its own products (with blocks of 128 keys TMEM has room for one buffer, and
+// softmax, P V and the next S of a tile came one after the other). m is raised
+// only when a score exceeds it by more than 2^8, so O in TMEM is rarely
+// rescaled.
 //
 // A sequence may end inside a key block. Keys behind it are masked by the
 // causal mask already; their V rows are zeroed in shared memory before the
@@ -42,10 +46,14 @@
 namespace {
 constexpr int kBM = 128;       // query rows per tile, keys per block
 constexpr int kHalf = kBM * 64 * 2;  // 16 KB: 64 columns x 128 rows, swizzled
-constexpr int kThreads = 384;
-constexpr int kSlots = 4;      // K/V ring
+constexpr int kSub = 64;       // keys per softmax step
+constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kItemWarp = 10;
+constexpr int kThreads = 352;
+constexpr int kMaxCtas = 160;  // (5 loads per lane of the items warp)
+constexpr int kItemCost = 1;   // what an item costs beside its key blocks, in blocks
+constexpr int kSlots = 5;      // K/V ring
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kIdescS = umma_idesc_bf16_f32(kBM, kBM, false);
+constexpr uint32_t kIdescS = umma_idesc_bf16_f32(kBM, kSub, false);
 template <int HD> constexpr int tile_bytes() { return kBM * HD * 2; }
 template <int HD> constexpr int off_bar() { return (2 + kSlots) * tile_bytes<HD>(); }
 template <int HD> constexpr int smem_bytes() { return off_bar<HD>() + 512 + 1024; }
@@ -73,52 +81,129 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return r;
 }
 
-// Item `i` of the launch (a whole warp calls it).
-__device__ Item find_item(const VarlenArgs& a, int i) {
-    const int lane = threadIdx.x & 31;
-    const int rows = a.pair_heads ? kBM : 2 * kBM, per_tile = a.pair_heads ? a.H / 2 : a.H;
-    const int k = i / per_tile, hh = i % per_tile;
-    auto depth = [&](int s) {  // tiles of sequence s; a sequence with bad bounds has none
+// This CTA's items, one after the other (a whole warp calls it).
+struct Dealer {
+    const VarlenArgs& a;
+    int rows, heads;        // rows of an item's tiles in a sequence, items per tile
+    int p, used;            // depth being dealt; CTAs that have an item (in order) while some have none
+    int load[kMaxCtas / 32];  // of CTAs lane, lane + 32, ...
+    int next, last;         // this CTA's items [next, last) of depth p
+
+    __device__ int depth(int s) const {  // of sequence s, in tiles; none where its bounds are bad
         if (s >= a.n_seq) return 0;
         const int b = a.cu[s], e = a.cu[s + 1];
         return b < 0 || e < b || e > a.total ? 0 : (e - b + rows - 1) / rows;
-    };
-    const int first = depth(lane);
-    auto each = [&](int s0) { return s0 ? depth(s0 + lane) : first; };
-    auto from = [&](int p) {  // tiles at depth p or more
+    }
+    __device__ explicit Dealer(const VarlenArgs& args) : a(args) {
+        rows = a.pair_heads ? kBM : 2 * kBM;
+        heads = a.pair_heads ? a.H / 2 : a.H;
+        int most = 0;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) most = max(most, depth(s0 + (threadIdx.x & 31)));
+        p = (int)__reduce_max_sync(0xffffffffu, most);
+        used = 0;
+        next = last = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxCtas / 32; ++i) load[i] = 0;
+    }
+    // The next depth's items over the CTAs.
+    __device__ void deal() {
+        const int lane = threadIdx.x & 31, G = gridDim.x, c = blockIdx.x;
+        --p;
         int n = 0;
-        for (int s0 = 0; s0 < a.n_seq; s0 += 32) n += max(0, each(s0) - p);
-        return (int)__reduce_add_sync(0xffffffffu, n);
-    };
-    Item it{};
-    it.head[0] = -1;
-    int lo = 0, hi = a.total / rows + 1;  // from(hi) == 0 <= k; the least p with from(p) <= k
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (from(mid) <= k) hi = mid;
-        else lo = mid + 1;
-    }
-    if (lo == 0) return it;  // k is behind the last tile
-    const int p = lo - 1;
-    int r = k - from(lo);    // the r-th sequence deeper than p
-    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-        const unsigned deep = __ballot_sync(0xffffffffu, each(s0) > p);
-        const int n = __popc(deep);
-        if (r < n) {
-            const int s = s0 + __fns(deep, 0, r + 1);
-            it.row0 = a.cu[s];
-            it.len = a.cu[s + 1] - it.row0;
-            it.head[0] = a.pair_heads ? 2 * hh : hh;
-            it.head[1] = a.pair_heads ? 2 * hh + 1 : hh;
-            it.kvh = it.head[0] / (a.H / a.Hkv);
-            it.tile[0] = a.pair_heads ? p : 2 * p;
-            it.tile[1] = a.pair_heads ? p : (2 * p + 1) * kBM < it.len ? 2 * p + 1 : -1;
-            return it;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) n += __popc(__ballot_sync(0xffffffffu, depth(s0 + lane) > p));
+        n *= heads;
+        const int w = (a.pair_heads ? p + 1 : 2 * p + 2) + kItemCost;
+        if (used + n <= G || used == 0) {  // to CTAs without one, or evenly over all
+            const int each = used ? 0 : n / G, more = used ? n : n % G;
+            const int mine = each + (c >= used && c < used + more);
+            next = each * c + min(max(c - used, 0), more);
+            last = next + mine;
+#pragma unroll
+            for (int i = 0; i < kMaxCtas / 32; ++i) {
+                const int k = 32 * i + lane;
+                if (k < G) load[i] += w * (each + (k >= used && k < used + more));
+            }
+            used = each ? G : used + more;
+            if (used >= G) used = G;
+            return;
         }
-        r -= n;
+        used = G;
+        // the level that takes the most items without passing n
+        int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxCtas / 32; ++i)
+            if (32 * i + lane < G) {
+                lo = min(lo, load[i]);
+                hi = max(hi, load[i]);
+            }
+        lo = (int)__reduce_min_sync(0xffffffffu, lo);
+        hi = (int)__reduce_max_sync(0xffffffffu, hi) + (n / G + 1) * w;
+        auto takes = [&](int level, int i) { return 32 * i + lane < G && load[i] < level ? (level - load[i]) / w : 0; };
+        auto total = [&](int level) {
+            int t = 0;
+#pragma unroll
+            for (int i = 0; i < kMaxCtas / 32; ++i) t += takes(level, i);
+            return (int)__reduce_add_sync(0xffffffffu, t);
+        };
+        while (lo < hi) {
+            const int mid = lo + (hi - lo + 1) / 2;
+            if (total(mid) <= n) lo = mid;
+            else hi = mid - 1;
+        }
+        // what is left goes to the CTAs that a level higher would give one, in order
+        int rest = n - total(lo), before = 0;
+        next = last = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxCtas / 32; ++i) {
+            int t = takes(lo, i);
+            const bool more = takes(lo + 1, i) > t;
+            const unsigned who = __ballot_sync(0xffffffffu, more);
+            if (more && __popc(who & ((1u << lane) - 1)) < rest) ++t;
+            rest = max(0, rest - __popc(who));
+            load[i] += t * w;
+            int inc = t;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            const int e = __shfl_sync(0xffffffffu, before + inc, c & 31), m = __shfl_sync(0xffffffffu, t, c & 31);
+            if (c / 32 == i) {
+                next = e - m;
+                last = e;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+        }
     }
-    return it;
-}
+    __device__ Item take() {
+        const int lane = threadIdx.x & 31;
+        Item it{};
+        it.head[0] = -1;
+        while (next == last) {
+            if (p == 0) return it;
+            deal();
+        }
+        const int r0 = next / heads, hh = next % heads;
+        ++next;
+        int r = r0;  // the r-th sequence deeper than p
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+            const unsigned deep = __ballot_sync(0xffffffffu, depth(s0 + lane) > p);
+            const int n = __popc(deep);
+            if (r < n) {
+                const int s = s0 + (int)__fns(deep, 0, r + 1);
+                it.row0 = a.cu[s];
+                it.len = a.cu[s + 1] - it.row0;
+                it.head[0] = a.pair_heads ? 2 * hh : hh;
+                it.head[1] = a.pair_heads ? 2 * hh + 1 : hh;
+                it.kvh = it.head[0] / (a.H / a.Hkv);
+                it.tile[0] = a.pair_heads ? p : 2 * p;
+                it.tile[1] = a.pair_heads ? p : (2 * p + 1) * kBM < it.len ? 2 * p + 1 : -1;
+                return it;
+            }
+            r -= n;
+        }
+        return it;
+    }
+};
 
 // 3-D tiled TMA load (no multicast): box {64 columns, 1 head, 128 rows}.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -126,6 +211,16 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
+}
+
+// One lane of a converged warp. (In a branch on elect.sync the compiler knows
+// that one thread is left, and an MMA's operands go straight to uniform
+// registers; in `if (lane == 0)` it loops over possible values of each, about
+// 100 cycles per 64-cycle product.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p = 0;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\t@e mov.s32 %0, 1;\n\t}" : "+r"(p));
+    return p != 0;
 }
 
 template <int HD>
@@ -143,13 +238,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + off_bar<HD>());
     uint64_t* q_full = bars + 0;
     uint64_t* q_empty = bars + 1;
-    uint64_t* s_full = bars + 2;              // [2] per tile
-    uint64_t* p_full = bars + 4;              // [2 tiles][2 halves]
-    uint64_t* o_done = bars + 8;              // [2]
-    uint64_t* o_free = bars + 10;             // [2]
-    uint64_t* item_full = bars + 12;          // [2]
-    uint64_t* item_empty = bars + 14;         // [2]
-    uint64_t* kv_full = bars + 16;            // [kSlots]
+    uint64_t* s_full = bars + 2;              // [2 tiles][2 buffers]
+    uint64_t* p_full = bars + 6;              // [2 tiles][2 buffers]
+    uint64_t* o_done = bars + 10;             // [2], a phase per P V but an item's last
+    uint64_t* o_last = bars + 12;             // [2], a phase per item
+    uint64_t* o_free = bars + 14;             // [2]
+    uint64_t* item_full = bars + 16;          // [2]
+    uint64_t* item_empty = bars + 18;         // [2]
+    uint64_t* kv_full = bars + 20;            // [kSlots]
     uint64_t* kv_empty = kv_full + kSlots;    // [kSlots]
     uint64_t* drain = kv_empty + kSlots;
     uint64_t* done = drain + 1;               // every warp finished (one arrival per warp)
@@ -164,13 +260,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[2 * i], 1);
+            mbar_init(&s_full[2 * i + 1], 1);
             mbar_init(&p_full[2 * i], 128);
             mbar_init(&p_full[2 * i + 1], 128);
             mbar_init(&o_done[i], 1);
+            mbar_init(&o_last[i], 1);
             mbar_init(&o_free[i], 128);
             mbar_init(&item_full[i], 1);
-            mbar_init(&item_empty[i], 10);  // TMA, MMA and 8 softmax warps
+            mbar_init(&item_empty[i], 2 + kSoftWarps);  // TMA, MMA and softmax warps
         }
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(&kv_full[i], 1);
@@ -182,12 +280,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     if (s_abort) return;
-    if (warp == 9) tmem_alloc(tslot, kTmemCols);
+    if (warp == kMmaWarp) tmem_alloc(tslot, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tslot;
-    // TMEM columns: S_A 0-127, O_A 128-255, S_B 256-383, O_B 384-511
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tslot, 0);
+    // TMEM columns: S_A 0-63 and 64-127, O_A 128-255, S_B 256-383, O_B 384-511
     const uint32_t tS[2] = {tmem, tmem + 256}, tO[2] = {tmem + 128, tmem + 384};
 
     // item n of this CTA, from the items warp
@@ -199,19 +297,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         return it.head[0] >= 0;
     };
     auto blocks = [](const Item& it, int t) { return it.tile[t] + 1; };  // key blocks of tile t (0: none)
+    // its half blocks: those with keys in the sequence
+    auto steps = [](const Item& it, int t) { return it.tile[t] < 0 ? 0 : 2 * it.tile[t] + (it.len - it.tile[t] * kBM > kSub ? 2 : 1); };
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 10) {
+    if (warp >= kSoftWarps) {
+        if (warp == kItemWarp) {
             // ------------------------------------------------------------ items
             // sequences with bad bounds
             if (blockIdx.x == 0)
                 for (int s = lane; s < a.n_seq; s += 32)
                     if (a.cu[s] < 0 || a.cu[s + 1] < a.cu[s] || a.cu[s + 1] > a.total) atomicOr(a.err, FORGE_DEVERR_BAD_INDEX);
+            Dealer dealer(a);
             for (int n = 0;; ++n) {
-                // the ordered items back and forth over the CTAs
-                const long long i = (long long)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                Item it = find_item(a, i > 0x7fffffff ? 0x7fffffff : (int)i);
+                const Item it = dealer.take();
                 if (!__all_sync(0xffffffffu, mbar_wait(&item_empty[n & 1], ((n >> 1) & 1) ^ 1, a.err))) break;
                 if (lane == 0) {
                     items[n & 1] = it;
@@ -220,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (it.head[0] < 0) break;
             }
-        } else if (warp == 8) {
+        } else if (warp == kTmaWarp) {
             // --------------------------------------------------------------- TMA
             Item it;
             int slot = 0;        // K/V tiles issued
@@ -258,84 +356,95 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (q_waits) mbar_wait(q_full, (q_waits - 1) & 1, a.err);
                 for (int i = max(0, slot - kSlots); i < slot; ++i) mbar_wait(&kv_full[i % kSlots], (i / kSlots) & 1, a.err);
             }
-        } else if (warp == 9) {
+        } else if (warp == kMmaWarp) {
             // ------------------------------------------------------ tensor cores
-            Item it;
-            int slot0 = 0;              // ring index of the item's K0
-            int np[2] = {0, 0};         // P blocks taken of each tile
-            int no[2] = {0, 0};         // items that used O of each tile
-            bool ok = true;
-            for (int n = 0; ok && take(n, it); ++n) {
-                const int nA = blocks(it, 0), nB = blocks(it, 1), nblk = max(nA, nB);
-                if (lane == 0) {
-                    auto slot_addr = [&](int b) { return sbase + (uint32_t)(kOffKV + ((slot0 + b) % kSlots) * kTile); };
-                    auto wait_kv = [&](int b) {
-                        const int i = slot0 + b;
-                        return mbar_wait(&kv_full[i % kSlots], (i / kSlots) & 1, a.err);
+            // (one thread, from here to the end: see elect_one)
+            if (elect_one()) {
+                const uint64_t desc_q = umma_desc_sw128(sbase, 16, 1024), desc_k = umma_desc_sw128(sbase + kOffKV, 16, 1024);
+                const uint64_t desc_v = umma_desc_sw128(sbase + kOffKV, kHalf, 1024);
+                uint32_t slot = 0, phase = 0;  // next ring slot and its parity
+                uint32_t par = 0;              // parities: bit 2 t + buffer: P taken; bit 4 + t: items that used O of tile t
+                bool ok = true;
+                for (uint32_t n = 0;; ++n) {
+                    if (!mbar_wait(&item_full[n & 1], (n >> 1) & 1, a.err)) break;
+                    const Item it = items[n & 1];
+                    mbar_arrive(&item_empty[n & 1]);
+                    if (it.head[0] < 0) break;
+                    // steps of both tiles; a tile's step j: S into buffer j % 2, later O += P V
+                    const int n0 = steps(it, 0), n1 = steps(it, 1), most = max(n0, n1);
+                    auto next_kv = [&](uint32_t& at) {
+                        at = slot;
+                        const uint32_t p = phase;
+                        if (++slot == kSlots) {
+                            slot = 0;
+                            phase ^= 1;
+                        }
+                        return mbar_wait(&kv_full[at], p, a.err);
                     };
-                    auto free_kv = [&](int b) { umma_commit(&kv_empty[(slot0 + b) % kSlots]); };
-                    auto issue_s = [&](int t, int j) {
-                        const uint32_t kb = slot_addr(2 * j), qb = sbase + (uint32_t)(t * kTile);
+                    auto issue_s = [&](int t, int buf, uint32_t ring) {
+                        const uint64_t q = desc_q + t * (kTile >> 4), k = desc_k + ring * (kTile >> 4) + buf * (kSub * 128 >> 4);
 #pragma unroll
                         for (int s = 0; s < HD / 16; ++s) {
-                            const uint32_t off = (uint32_t)((s >> 2) * kHalf + (s & 3) * 32);
-                            umma_bf16(tS[t], umma_desc_sw128(qb + off, 16, 1024), umma_desc_sw128(kb + off, 16, 1024), kIdescS,
-                                      s > 0 ? 1u : 0u);
+                            const uint32_t off = ((s >> 2) * kHalf + (s & 3) * 32) >> 4;
+                            umma_bf16(tS[t] + kSub * buf, q + off, k + off, kIdescS, s > 0);
                         }
-                        umma_commit(&s_full[t]);
+                        umma_commit(&s_full[2 * t + buf]);
                     };
-                    // O += P V in two halves as P arrives; P (A operand) lies in TMEM over S, 8 columns per 16 keys
-                    auto issue_pv = [&](int t, int j, bool last) {
-                        const uint32_t vb = slot_addr(2 * j + 1);
-                        for (int hf = 0; hf < 2; ++hf) {
-                            if (!mbar_wait(&p_full[2 * t + hf], np[t] & 1, a.err)) return false;
-                            tc_fence_after();
+                    // P (A operand) lies in TMEM over S, 8 columns per 16 keys
+                    auto issue_pv = [&](int t, int buf, uint32_t ring, bool more, bool last) {
+                        if (!mbar_wait(&p_full[2 * t + buf], (par >> (2 * t + buf)) & 1, a.err)) return false;
+                        par ^= 1u << (2 * t + buf);
+                        tc_fence_after();
+                        const uint64_t v = desc_v + ring * (kTile >> 4) + buf * (kSub * 128 >> 4);
 #pragma unroll
-                            for (int s = 4 * hf; s < 4 * hf + 4; ++s)
-                                umma_bf16_ta(tO[t], tS[t] + (uint32_t)(8 * s), umma_desc_sw128(vb + (uint32_t)s * 2048u, kHalf, 1024),
-                                             kIdescO, (j > 0 || s > 0) ? 1u : 0u);
-                        }
-                        ++np[t];
-                        if (last) umma_commit(&o_done[t]);
+                        for (int s = 0; s < kSub / 16; ++s)
+                            umma_bf16_ta(tO[t], tS[t] + kSub * buf + 8 * s, v + s * (2048 >> 4), kIdescO, more || s > 0);
+                        umma_commit(last ? &o_last[t] : &o_done[t]);
                         return true;
                     };
-                    ok = mbar_wait(q_full, n & 1, a.err) && wait_kv(0);
-                    if (ok) {
-                        tc_fence_after();
-                        issue_s(0, 0);
-                        if (nB) issue_s(1, 0);
-                        free_kv(0);
-                        if (nblk == 1) umma_commit(q_empty);
-                    }
+                    uint32_t k_at = 0, v_at = 0;
+                    if (!mbar_wait(q_full, n & 1, a.err) || !next_kv(k_at)) break;
+                    tc_fence_after();
+                    if (n0) issue_s(0, 0, k_at);
+                    if (n1) issue_s(1, 0, k_at);
+                    if (n0 > 1) issue_s(0, 1, k_at);
+                    if (n1 > 1) issue_s(1, 1, k_at);
+                    umma_commit(&kv_empty[k_at]);
+                    if (most <= 2) umma_commit(q_empty);  // the item's last S is issued
                     // the softmax warps have taken the last item's O
-                    for (int t = 0; t < 2; ++t)
-                        if (ok && (t ? nB : nA)) {
-                            ok = mbar_wait(&o_free[t], (no[t] & 1) ^ 1, a.err);
-                            ++no[t];
-                        }
-                    for (int j = 0; ok && j < nblk; ++j) {
-                        ok = wait_kv(2 * j + 1);
-                        if (ok && j < nA) ok = issue_pv(0, j, j + 1 == nA);
-                        // tile A's next S overlaps tile B's softmax of this block
-                        const bool nextA = j + 1 < nA, nextB = j + 1 < nB;
-                        if (ok && (nextA || nextB)) {
-                            ok = wait_kv(2 * j + 2);
-                            if (!ok) break;
-                            tc_fence_after();
-                            if (nextA) issue_s(0, j + 1);
-                        }
-                        if (ok && j < nB) ok = issue_pv(1, j, j + 1 == nB);
-                        if (!ok) break;
-                        free_kv(2 * j + 1);
-                        if (nextB) issue_s(1, j + 1);
-                        if (nextA || nextB) free_kv(2 * j + 2);
-                        if (j + 2 == nblk) umma_commit(q_empty);  // the item's last S is issued
+                    if (n0) {
+                        ok = mbar_wait(&o_free[0], ((par >> 4) & 1) ^ 1, a.err);
+                        par ^= 1u << 4;
                     }
+                    if (ok && n1) {
+                        ok = mbar_wait(&o_free[1], ((par >> 5) & 1) ^ 1, a.err);
+                        par ^= 1u << 5;
+                    }
+                    for (int j = 0; ok && j < most; j += 2) {
+                        const bool more_k = j + 2 < most;
+                        if (!next_kv(v_at)) { ok = false; break; }
+                        bool have_k = false;
+#pragma unroll
+                        for (int buf = 0; buf < 2; ++buf)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const int nt = t ? n1 : n0;
+                                if (ok && j + buf < nt) {
+                                    ok = issue_pv(t, buf, v_at, j + buf > 0, j + buf + 1 == nt);
+                                    if (ok && more_k && !have_k) {
+                                        have_k = ok = next_kv(k_at);
+                                        tc_fence_after();
+                                    }
+                                    if (ok && j + buf + 2 < nt) issue_s(t, buf, k_at);
+                                }
+                            }
+                        if (!ok) break;
+                        umma_commit(&kv_empty[v_at]);
+                        if (more_k) umma_commit(&kv_empty[k_at]);
+                        if (more_k && j + 4 >= most) umma_commit(q_empty);
+                    }
+                    if (!ok) break;
                 }
-                slot0 += 2 * nblk;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-            }
-            if (lane == 0) {
                 umma_commit(drain);
                 mbar_wait(drain, 0, a.err);
             }
@@ -343,63 +452,72 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2;                  // tile 0 (A) or 1 (B)
         const int r = threadIdx.x & 127;          // query row within the tile
         const uint32_t lrow = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tSm = tS[t] + lrow, tOm = tO[t] + lrow;
         const float c = a.scale_log2;
         Item it;
-        int ns = 0;      // S blocks taken
-        int no = 0;      // items that used O
-        int slot0 = 0;   // ring index of the item's K0
+        uint32_t ns[2] = {0, 0};  // parity of the S taken from either buffer
+        uint32_t np = 0;          // P V of this tile so far
+        uint32_t no = 0;          // items that had this tile
+        int slot0 = 0;            // ring index of the item's K0
         for (int n = 0; take(n, it); ++n) {
-            const int nmine = blocks(it, t), nblk = max(blocks(it, 0), blocks(it, 1));
-            const int qt = it.tile[t];
+            const int nmine = steps(it, t), qt = it.tile[t];
             // Running max in log2 units (m = max * c), raised only when a new score exceeds it by more than 8 (P stays
             // below 2^8, exact enough in bf16 and fp32), so O in TMEM is rescaled rarely; l and O refer to the same m.
             float m = -INFINITY, l = 0.f;
             bool ok = nmine > 0;
-            for (int j = 0; j < nmine; ++j, ++ns) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], ns & 1, a.err))) { ok = false; break; }
+            for (int j = 0; j < nmine; ++j, np += j < nmine) {  // (the last P V has a barrier of its own)
+                const int buf = j & 1;
+                if (!__all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + buf], buf ? ns[1] : ns[0], a.err))) { ok = false; break; }
+                if (buf) ns[1] ^= 1;
+                else ns[0] ^= 1;
                 tc_fence_after();
-                uint32_t sv[4][32];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(tSm + 32 * q, sv[q]);
+                const uint32_t tSb = tSm + kSub * buf;
+                uint32_t sv[2][32];
+                tmem_ld32(tSb, sv[0]);
+                tmem_ld32(tSb + 32, sv[1]);
                 tmem_wait_ld();
-                if (j == qt) {  // the diagonal block
+                if (j >= 2 * qt) {  // the diagonal block
+                    const int first = kSub * buf;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                    for (int q = 0; q < 2; ++q)
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (32 * q + i > r) sv[q][i] = 0xFF800000u;
+                            if (first + 32 * q + i > r) sv[q][i] = 0xFF800000u;
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
                         mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sv[q][i]), __uint_as_float(sv[q][i + 1]));
                 const float mxc = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c;
-                const bool raise = mxc > m + 8.0f || m == -INFINITY;
-                const float m_new = raise ? mxc : m;
-                const float alpha = raise && j > 0 ? ex2(m - m_new) : 1.0f;
-                // (S of block j is complete, so is O += P V of block j - 1, issued before it)
-                if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                const bool raise = mxc > m + 8.0f || j == 0;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float alpha = raise && j > 0 ? ex2(m - mxc) : 1.0f;
+                    m = raise ? mxc : m;
+                    l *= alpha;
+                    if (j > 0) {
+                        // P V of the step before has to be in O
+                        if (!__all_sync(0xffffffffu, mbar_wait(&o_done[t], (np - 1) & 1, a.err))) { ok = false; break; }
+                        tc_fence_after();
 #pragma unroll
-                    for (int q = 0; q < HD / 32; ++q) {
-                        uint32_t ov[32];
-                        tmem_ld32(tOm + 32 * q, ov);
-                        tmem_wait_ld();
+                        for (int q = 0; q < HD / 32; ++q) {
+                            uint32_t ov[32];
+                            tmem_ld32(tOm + 32 * q, ov);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-                        tmem_st32(tOm + 32 * q, ov);
+                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                            tmem_st32(tOm + 32 * q, ov);
+                        }
                     }
                 }
-                const F2 c2(c, c), nm2(-m_new, -m_new);
+                const F2 c2(c, c), nm2(-m, -m);
                 F2 sum(0.f, 0.f);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < 2; ++q) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -408,36 +526,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                         sum = sum + p;
                         pk[e] = pack_bf16x2(p.x(), p.y());
                     }
-                    tmem_st16(tSm + 16 * q, pk);
-                    if (q == 1) {
-                        tmem_wait_st();
-                        // the sequence ends inside the block: V rows behind its end count for nothing
-                        const int valid = it.len - j * kBM;
-                        if (valid < kBM) {
-                            const int b = slot0 + 2 * j + 1;
-                            mbar_wait(&kv_full[b % kSlots], (b / kSlots) & 1, a.err);
-                            if (r >= valid) {
-                                uint4* row = reinterpret_cast<uint4*>(base + kOffKV + (b % kSlots) * kTile + r * 128);
-#pragma unroll
-                                for (int h2 = 0; h2 < kNH; ++h2)
-#pragma unroll
-                                    for (int i = 0; i < 8; ++i) row[h2 * (kHalf / 16) + i] = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async_smem();
-                        }
-                        tc_fence_before();
-                        mbar_arrive(&p_full[2 * t]);
-                    }
+                    tmem_st16(tSb + 16 * q, pk);
                 }
-                l = l * alpha + (sum.x() + sum.y());
-                m = m_new;
+                l += sum.x() + sum.y();
+                // the sequence ends inside the half block: V rows behind its end count for nothing
+                const int valid = it.len - j * kSub;
+                if (valid < kSub) {
+                    const int b = slot0 + (j | 1), row = r & (kSub - 1), half = r / kSub;
+                    mbar_wait(&kv_full[b % kSlots], (b / kSlots) & 1, a.err);
+                    if (row >= valid && half < kNH) {
+                        uint4* z = reinterpret_cast<uint4*>(base + kOffKV + (b % kSlots) * kTile + half * kHalf + (kSub * buf + row) * 128);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) z[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[2 * t + 1]);
+                mbar_arrive(&p_full[2 * t + buf]);
             }
-            slot0 += 2 * nblk;
+            slot0 += 2 * max(blocks(it, 0), blocks(it, 1));
             if (nmine == 0) continue;
-            if (!ok || !__all_sync(0xffffffffu, mbar_wait(&o_done[t], no & 1, a.err))) break;
+            if (!ok || !__all_sync(0xffffffffu, mbar_wait(&o_last[t], no & 1, a.err))) break;
             ++no;
             tc_fence_after();
             const float inv = 1.0f / l;
@@ -469,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(done);
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         mbar_wait(done, 0, a.err);
         __syncwarp();
         tc_fence_after();
@@ -532,7 +642,7 @@ extern "C" FORGE_API int forge_flash_prefill_varlen(const uint16_t* q, int64_t l
     a.cu = cu_seqlens; a.n_seq = n_seq; a.total = total; a.H = H; a.Hkv = Hkv;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.o = o; a.ldo = ldo; a.lse = lse; a.err = err;
-    const int sms = forge_sm_count();
+    const int sms = forge_sm_count() < kMaxCtas ? forge_sm_count() : kMaxCtas;
     const unsigned grid = (unsigned)(items < sms ? items : sms);
     if (hd == 128) k_prefill_varlen<128><<<grid, kThreads, smem_bytes<128>(), (cudaStream_t)stream>>>(mq, mk, mv, a);
     else k_prefill_varlen<64><<<grid, kThreads, smem_bytes<64>(), (cudaStream_t)stream>>>(mq, mk, mv, a);

@@ -10,11 +10,13 @@
 // same blocks, and a short prompt fills both), else two consecutive tiles of
 // one head. CTAs are persistent, one per SM. Items are dealt out longest
 // first: for every depth (position of the tile in its sequence) from the
-// deepest, its items raise the CTAs' loads to a common level. Every CTA works
-// this out for itself, in a warp of its own that runs ahead of the others, so
-// that any mix of lengths is even without a table, a counter or a second
-// launch (dealing the sorted items out back and forth instead took 1.4 times
-// as long for 8 prompts of 1 to 1024 tokens).
+// deepest, its items raise the CTAs' loads to a common level.
+// Heads are dealt a group at a time, as many as keep their K and V in half of
+// L2 (for 8 prompts of 4096 with 32 KV heads all heads at once read HBM 2.6
+// times and took 1.11 ms instead of 0.99). Every CTA works this out for
+// itself, in a warp of its own that runs ahead of the others, so that any mix
+// of lengths is even without a table, a counter or a second launch (dealing
+// the sorted items out back and forth instead took up to 1.4 times as long).
 //
 //   warps 0-3 / 4-7    softmax of tile A / B, one thread per query row
 //   warp 8             TMA: Q of both tiles, K and V through a 5-slot ring
@@ -61,6 +63,7 @@ template <int HD> constexpr int smem_bytes() { return off_bar<HD>() + 512 + 1024
 struct VarlenArgs {
     const int32_t* cu;
     int n_seq, total, H, Hkv;
+    int group;            // items per tile (heads or pairs of them) whose K/V are worked on together
     int pair_heads;       // items are (tile, head pair), else (tile pair, head)
     float scale_log2;     // log2(e) / sqrt(hd)
     uint16_t* o;
@@ -81,11 +84,33 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return r;
 }
 
+// 2^x on the FMA pipe, two values: x = i + f with i the nearest integer (the
+// sum with 1.5 2^23 holds it in its low bits), a polynomial of degree 4 in f
+// in [-1/2, 1/2] (Remez fit with p(0) = 1, relative error 2.9e-6, mean
+// 2e-7: P is rounded to bf16 and its sum averages it), i added to the
+// exponent. Below -127 (masked scores) exactly 0.
+__device__ __forceinline__ F2 exp2_fma(F2 x) {
+    const F2 c(fmaxf(x.x(), -127.f), fmaxf(x.y(), -127.f)), magic(12582912.f, 12582912.f);
+    const F2 y = c + magic, i = y + F2(-12582912.f, -12582912.f), f = fma2(i, F2(-1.f, -1.f), c);
+    F2 p = fma2(f, F2(0.009582853f, 0.009582853f), F2(0.055906426f, 0.055906426f));
+    p = fma2(p, f, F2(0.240240991f, 0.240240991f));
+    p = fma2(p, f, F2(0.693124175f, 0.693124175f));
+    p = fma2(p, f, F2(1.f, 1.f));
+    return F2(__int_as_float(__float_as_int(p.x()) + (__float_as_int(y.x()) << 23)),
+              __int_as_float(__float_as_int(p.y()) + (__float_as_int(y.y()) << 23)));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // This CTA's items, one after the other (a whole warp calls it).
 struct Dealer {
     const VarlenArgs& a;
     int rows, heads;        // rows of an item's tiles in a sequence, items per tile
-    int p, used;            // depth being dealt; CTAs that have an item (in order) while some have none
+    int group, h0, hn;      // items per tile dealt together; those in hand: [h0, h0 + hn)
+    int deepest, p, used;   // the deepest tile, the depth being dealt; CTAs that have an item while some have none
     int load[kMaxCtas / 32];  // of CTAs lane, lane + 32, ...
     int next, last;         // this CTA's items [next, last) of depth p
 
@@ -94,12 +119,17 @@ struct Dealer {
         const int b = a.cu[s], e = a.cu[s + 1];
         return b < 0 || e < b || e > a.total ? 0 : (e - b + rows - 1) / rows;
     }
-    __device__ explicit Dealer(const VarlenArgs& args) : a(args) {
+    __device__ explicit Dealer(const VarlenArgs& args) : a(args) {}
+    __device__ void start() {
         rows = a.pair_heads ? kBM : 2 * kBM;
         heads = a.pair_heads ? a.H / 2 : a.H;
         int most = 0;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) most = max(most, depth(s0 + (threadIdx.x & 31)));
-        p = (int)__reduce_max_sync(0xffffffffu, most);
+        deepest = (int)__reduce_max_sync(0xffffffffu, most);
+        group = a.group;
+        p = deepest;
+        h0 = 0;
+        hn = min(group, heads);
         used = 0;
         next = last = 0;
 #pragma unroll
@@ -111,7 +141,7 @@ struct Dealer {
         --p;
         int n = 0;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) n += __popc(__ballot_sync(0xffffffffu, depth(s0 + lane) > p));
-        n *= heads;
+        n *= hn;
         const int w = (a.pair_heads ? p + 1 : 2 * p + 2) + kItemCost;
         if (used + n <= G || used == 0) {  // to CTAs without one, or evenly over all
             const int each = used ? 0 : n / G, more = used ? n : n % G;
@@ -128,31 +158,42 @@ struct Dealer {
             return;
         }
         used = G;
-        // the level that takes the most items without passing n
-        int lo = 0x7fffffff, hi = 0;
+        // The level that takes the most items without passing n. (In fp32, the same in every CTA: what matters is that
+        // all agree.) It is the mean of what will be there, or less where some loads lie above it.
+        int low = 0x7fffffff, high = 0, sum = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxCtas / 32; ++i)
+            if (32 * i + lane < G) low = min(low, load[i]);
+        low = (int)__reduce_min_sync(0xffffffffu, low);
 #pragma unroll
         for (int i = 0; i < kMaxCtas / 32; ++i)
             if (32 * i + lane < G) {
-                lo = min(lo, load[i]);
-                hi = max(hi, load[i]);
+                load[i] -= low;
+                high = max(high, load[i]);
+                sum += load[i];
             }
-        lo = (int)__reduce_min_sync(0xffffffffu, lo);
-        hi = (int)__reduce_max_sync(0xffffffffu, hi) + (n / G + 1) * w;
-        auto takes = [&](int level, int i) { return 32 * i + lane < G && load[i] < level ? (level - load[i]) / w : 0; };
+        sum = (int)__reduce_add_sync(0xffffffffu, sum);
+        high = (int)__reduce_max_sync(0xffffffffu, high);
+        const float inv = 1.0f / (float)w;
+        auto takes = [&](int level, int i) {
+            return 32 * i + lane < G && load[i] < level ? (int)(((float)(level - load[i]) + 0.5f) * inv) : 0;
+        };
         auto total = [&](int level) {
             int t = 0;
 #pragma unroll
             for (int i = 0; i < kMaxCtas / 32; ++i) t += takes(level, i);
             return (int)__reduce_add_sync(0xffffffffu, t);
         };
+        const int mean = (int)min(((long long)sum + (long long)n * w) / G, 0x3fffffffll);
+        int lo = 0, hi = max(high, mean) + w + 1;
+        if (mean > 1 && total(mean - 1) <= n) lo = mean - 1;
         while (lo < hi) {
             const int mid = lo + (hi - lo + 1) / 2;
             if (total(mid) <= n) lo = mid;
             else hi = mid - 1;
         }
         // what is left goes to the CTAs that a level higher would give one, in order
-        int rest = n - total(lo), before = 0;
-        next = last = 0;
+        int rest = n - total(lo), before = 0, mine = 0;
 #pragma unroll
         for (int i = 0; i < kMaxCtas / 32; ++i) {
             int t = takes(lo, i);
@@ -161,28 +202,26 @@ struct Dealer {
             if (more && __popc(who & ((1u << lane) - 1)) < rest) ++t;
             rest = max(0, rest - __popc(who));
             load[i] += t * w;
-            int inc = t;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += u;
-            }
-            const int e = __shfl_sync(0xffffffffu, before + inc, c & 31), m = __shfl_sync(0xffffffffu, t, c & 31);
-            if (c / 32 == i) {
-                next = e - m;
-                last = e;
-            }
-            before += __shfl_sync(0xffffffffu, inc, 31);
+            if (32 * i + lane < c) before += t;
+            if (32 * i + lane == c) mine = t;
         }
+        next = (int)__reduce_add_sync(0xffffffffu, before);
+        last = next + (int)__reduce_add_sync(0xffffffffu, mine);
     }
     __device__ Item take() {
         const int lane = threadIdx.x & 31;
         Item it{};
         it.head[0] = -1;
         while (next == last) {
-            if (p == 0) return it;
+            if (p == 0) {  // the next heads
+                h0 += hn;
+                hn = min(group, heads - h0);
+                p = deepest;
+                if (hn <= 0 || p == 0) return it;
+            }
             deal();
         }
-        const int r0 = next / heads, hh = next % heads;
+        const int r0 = next / hn, hh = h0 + next % hn;
         ++next;
         int r = r0;  // the r-th sequence deeper than p
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
@@ -278,6 +317,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(done, kThreads / 32);
         fence_mbar_init();
     }
+    Dealer dealer(a);
+    Item first{};
+    if (warp == kItemWarp) {  // (its loads run beside the barriers' and TMEM's setup)
+        dealer.start();
+        first = dealer.take();
+    }
+    if (warp == kTmaWarp && lane < 3) {
+        const CUtensorMap* m = lane == 0 ? &tq : lane == 1 ? &tk : &tv;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
     __syncthreads();
     if (s_abort) return;
     if (warp == kMmaWarp) tmem_alloc(tslot, kTmemCols);
@@ -307,9 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (blockIdx.x == 0)
                 for (int s = lane; s < a.n_seq; s += 32)
                     if (a.cu[s] < 0 || a.cu[s + 1] < a.cu[s] || a.cu[s + 1] > a.total) atomicOr(a.err, FORGE_DEVERR_BAD_INDEX);
-            Dealer dealer(a);
             for (int n = 0;; ++n) {
-                const Item it = dealer.take();
+                const Item it = n ? dealer.take() : first;
                 if (!__all_sync(0xffffffffu, mbar_wait(&item_empty[n & 1], ((n >> 1) & 1) ^ 1, a.err))) break;
                 if (lane == 0) {
                     items[n & 1] = it;
@@ -492,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
-                        mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sv[q][i]), __uint_as_float(sv[q][i + 1]));
-                const float mxc = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c;
+                        mx4[(i >> 1) & 3] = max3_nan(mx4[(i >> 1) & 3], __uint_as_float(sv[q][i]), __uint_as_float(sv[q][i + 1]));
+                const float mxc = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
                 const bool raise = mxc > m + 8.0f || j == 0;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float alpha = raise && j > 0 ? ex2(m - mxc) : 1.0f;
@@ -522,13 +570,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const F2 x = fma2(F2(__uint_as_float(sv[q][2 * e]), __uint_as_float(sv[q][2 * e + 1])), c2, nm2);
-                        const F2 p(ex2(x.x()), ex2(x.y()));
+                        // of 4 pairs, 1 on the FMA pipe (the exp2 unit takes 8 cycles for a warp's value)
+                        const F2 p = e % 4 == 1 ? exp2_fma(x) : F2(ex2(x.x()), ex2(x.y()));
                         sum = sum + p;
                         pk[e] = pack_bf16x2(p.x(), p.y());
                     }
                     tmem_st16(tSb + 16 * q, pk);
                 }
-                l += sum.x() + sum.y();
+                l += isnan(mxc) ? NAN : sum.x() + sum.y();  // (a NaN score makes the row NaN)
                 // the sequence ends inside the half block: V rows behind its end count for nothing
                 const int valid = it.len - j * kSub;
                 if (valid < kSub) {
@@ -642,6 +691,11 @@ extern "C" FORGE_API int forge_flash_prefill_varlen(const uint16_t* q, int64_t l
     a.cu = cu_seqlens; a.n_seq = n_seq; a.total = total; a.H = H; a.Hkv = Hkv;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.o = o; a.ldo = ldo; a.lse = lse; a.err = err;
+    // half of L2 for the K and V of a group's heads
+    const int64_t kv_bytes = (int64_t)total * hd * 4, per_tile = a.pair_heads ? H / 2 : H;
+    const int64_t kv_heads = (60ll << 20) / kv_bytes;
+    const int64_t group = (kv_heads < 1 ? 1 : kv_heads) * per_tile / Hkv;
+    a.group = (int)(group < 1 ? 1 : group < per_tile ? group : per_tile);
     const int sms = forge_sm_count() < kMaxCtas ? forge_sm_count() : kMaxCtas;
     const unsigned grid = (unsigned)(items < sms ? items : sms);
     if (hd == 128) k_prefill_varlen<128><<<grid, kThreads, smem_bytes<128>(), (cudaStream_t)stream>>>(mq, mk, mv, a);

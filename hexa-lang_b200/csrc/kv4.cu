@@ -4,7 +4,14 @@
 // x / s to the nearest integer, halves away from zero, clamped to -7..7, plus
 // 7 (the rule of k_q4_quantize, weights.cu). A group with a value that is not
 // finite gets a NaN scale.
+//
+// Bound by HBM for prompts, by latency for a decode step's rows. A CTA takes
+// the K or the V of one row, so the row's place in the cache is looked up once;
+// a thread takes 8 dims (16 bytes of bf16, 4 bytes of codes, 32 bytes of fp32),
+// 8 neighbouring threads a group, and a row's loads are issued before its
+// place is known.
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "forge_internal.h"
 #include "../../include/forge_b200.h"
 #include "../../include/forge_kv4.h"
@@ -22,79 +29,152 @@ struct RowArgs {
     uint32_t* err;
 };
 
-// Index of the cache row (slab * Hkv + head) * rows + row, or -1 (error word).
-__device__ int64_t cache_row(const ForgeKv4& c, int s, int p, int head, uint32_t* err) {
+// Index of the cache row (slab * Hkv) * rows + row of head 0, or -1 (error word).
+__device__ int64_t cache_row(const ForgeKv4& c, int s, int p, uint32_t* err) {
     const int cap = c.table ? c.max_pages * c.page_tokens : c.lmax;
-    if (s < 0 || s >= c.n_seq || p >= cap) {
-        atomicOr(err, FORGE_DEVERR_BAD_INDEX);
-        return -1;
+    if (s >= 0 && s < c.n_seq && p < cap) {
+        if (!c.table) return (int64_t)s * c.n_kv_head * c.lmax + p;
+        const int pg = c.table[(int64_t)s * c.max_pages + p / c.page_tokens];
+        if ((unsigned)pg < (unsigned)c.num_pages) return (int64_t)pg * c.n_kv_head * c.page_tokens + p % c.page_tokens;
     }
-    if (!c.table) return ((int64_t)s * c.n_kv_head + head) * c.lmax + p;
-    const int pg = c.table[(int64_t)s * c.max_pages + p / c.page_tokens];
-    if ((unsigned)pg >= (unsigned)c.num_pages) {
-        atomicOr(err, FORGE_DEVERR_BAD_INDEX);
-        return -1;
-    }
-    return ((int64_t)pg * c.n_kv_head + head) * c.page_tokens + p % c.page_tokens;
+    if (threadIdx.x == 0) atomicOr(err, FORGE_DEVERR_BAD_INDEX);
+    return -1;
 }
 
-// One warp per (row, head, K or V, group): lane l holds dims 2l, 2l + 1.
-__global__ void __launch_bounds__(256) k_kv4_append(const RowArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int ng = a.c.head_dim / kGroup;
-    const int64_t n = (int64_t)a.n_rows * a.c.n_kv_head * 2 * ng;
-    for (int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; w < n; w += (int64_t)gridDim.x * 8) {
-        const int g = (int)(w % ng), kv = (int)(w / ng % 2), h = (int)(w / ng / 2 % a.c.n_kv_head);
-        const int64_t r = w / ng / 2 / a.c.n_kv_head;
-        const int p = a.pos[r];
-        if (p < 0) continue;
-        const int64_t row = cache_row(a.c, a.seq ? a.seq[r] : (int)r, p, h, a.err);
-        if (row < 0) continue;
-        const uint32_t x2 = *reinterpret_cast<const uint32_t*>((kv ? a.v : a.k) + r * a.ld + h * a.c.head_dim + g * kGroup + 2 * lane);
-        const float x[2] = {bf16_lo_f32(x2), bf16_hi_f32(x2)};
-        float m = fmaxf(fabsf(x[0]), fabsf(x[1]));
-        if (!(fabsf(x[0]) <= 3.4e38f) || !(fabsf(x[1]) <= 3.4e38f)) m = INFINITY;
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        uint16_t sb = m == INFINITY ? 0x7FC0 : f32_to_bf16_bits(m / 7.0f);
-        if (sb == 0) sb = 0x3F80;
-        const float s = bf16_bits_to_f32(sb);
-        uint32_t byte = 0;
-        for (int i = 0; i < 2; ++i) {
-            const float q = m == INFINITY ? 0.f : x[i] / s;
-            const int c = max(-7, min(7, (int)(q + (q < 0.f ? -0.5f : 0.5f)))) + 7;
-            byte |= (uint32_t)c << (4 * i);
+constexpr int kThreads = 128;
+constexpr int kAhead = 4;  // chunks of 8 dims a thread has in flight
+
+// Codes of 8 dims (even dim in a byte's low nibble) of a group shared by 8
+// neighbouring lanes, and the group's scale.
+//
+// Rounding x / s (halves away from zero) without a division: x and s are bf16
+// values, so x / s is a half exactly or at least 2^-10 away from one (a
+// difference of products of 8-bit integers over 2 s). x inv with inv = 1 / s
+// to 2^-22, made larger by 2^-14, lies beyond a half that x / s meets and,
+// below 7.5, not beyond one that it does not; an fma onto 1.5 2^23 + 7 then
+// rounds it to the integer and leaves the code in the low bits. amax / 7 in
+// the same way: the nearest bf16 of amax (1 / 7) is that of amax / 7, which
+// is a bf16 value or at least 2^-13 of itself from a half between two.
+__device__ __forceinline__ uint32_t quantise8(const uint4& x, uint16_t& scale) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t amax = max(m & 0xffffu, m >> 16);  // bf16 bits; infinity and NaN from 0x7F80 on
+    scale = f32_to_bf16_bits(bf16_bits_to_f32((uint16_t)amax) * (1.0f / 7.0f));
+    if (scale == 0) scale = 0x3F80;
+    const float s = bf16_bits_to_f32(scale);
+    const bool tiny = s < 0x1p-100f;  // (1 / s may be no fp32 number, and amax / s above 7.5)
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(tiny ? s * 0x1p64f : s));
+    inv *= 1.0f + 0x1p-14f;
+    uint32_t codes = 0;
+    if (!__any_sync(0xffffffffu, tiny)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = fmaf(i & 1 ? bf16_hi_f32(w[i / 2]) : bf16_lo_f32(w[i / 2]), inv, 12582919.0f);
+            codes += (__float_as_uint(y) - 0x4B400000u) << (4 * i);
         }
-        (kv ? a.c.v : a.c.k)[row * (a.c.head_dim / 2) + g * (kGroup / 2) + lane] = (uint8_t)byte;
-        if (lane == 0) (kv ? a.c.vs : a.c.ks)[row * ng + g] = sb;
-    }
-}
-
-// One warp per (row, head, K or V, group): lane l writes dims 2l, 2l + 1.
-__global__ void __launch_bounds__(256) k_kv4_read(const RowArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int ng = a.c.head_dim / kGroup;
-    const int64_t n = (int64_t)a.n_rows * a.c.n_kv_head * 2 * ng;
-    for (int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; w < n; w += (int64_t)gridDim.x * 8) {
-        const int g = (int)(w % ng), kv = (int)(w / ng % 2), h = (int)(w / ng / 2 % a.c.n_kv_head);
-        const int64_t r = w / ng / 2 / a.c.n_kv_head;
-        const int p = a.pos[r];
-        if (p < 0) continue;
-        const int64_t row = cache_row(a.c, a.seq ? a.seq[r] : (int)r, p, h, a.err);
-        float2 o = make_float2(NAN, NAN);
-        if (row >= 0) {
-            const uint32_t byte = (kv ? a.c.v : a.c.k)[row * (a.c.head_dim / 2) + g * (kGroup / 2) + lane];
-            const float s = bf16_bits_to_f32((kv ? a.c.vs : a.c.ks)[row * ng + g]);
-            o = make_float2((float)((int)(byte & 15) - 7) * s, (float)((int)(byte >> 4) - 7) * s);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = (i & 1 ? bf16_hi_f32(w[i / 2]) : bf16_lo_f32(w[i / 2])) * (tiny ? 0x1p64f : 1.0f);
+            const float y = fminf(fmaxf(fmaf(v, inv, 12582919.0f), 12582912.0f), 12582926.0f);
+            codes += (__float_as_uint(y) - 0x4B400000u) << (4 * i);
         }
-        *reinterpret_cast<float2*>((kv ? a.vo : a.ko) + r * a.ld + h * a.c.head_dim + g * kGroup + 2 * lane) = o;
+    }
+    if (amax >= 0x7F80u) {
+        scale = 0x7FC0;
+        codes = 0x77777777u;
+    }
+    return codes;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads) k_kv4_append(const RowArgs a) {
+    constexpr int kPer = HD / 8;  // chunks a head
+    const int64_t r = blockIdx.x;
+    const bool v = blockIdx.y;
+    const int chunks = a.c.n_kv_head * kPer;
+    const uint4* x = reinterpret_cast<const uint4*>((v ? a.v : a.k) + r * a.ld);
+    uint4 in[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i * kThreads + (int)threadIdx.x < chunks) in[i] = __ldcs(x + i * kThreads + threadIdx.x);
+    const int p = a.pos[r];
+    if (p < 0) return;
+    const int64_t row = cache_row(a.c, a.seq ? a.seq[r] : (int)r, p, a.err);
+    if (row < 0) return;
+    const int64_t head_rows = a.c.table ? a.c.page_tokens : a.c.lmax;  // from a head to the next
+    uint32_t* codes = reinterpret_cast<uint32_t*>(v ? a.c.v : a.c.k) + row * kPer;
+    uint16_t* scales = (v ? a.c.vs : a.c.ks) + row * (HD / kGroup);
+    for (int base = 0; base < chunks; base += kAhead * kThreads) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (base + i * kThreads >= chunks) break;  // (the whole CTA: a group's lanes shuffle)
+            const int c = base + i * kThreads + (int)threadIdx.x;
+            uint16_t s;
+            const uint32_t q = quantise8(in[i], s);
+            if (c < chunks) {
+                const int64_t at = (c / kPer) * head_rows;
+                const int d = c % kPer;
+                codes[at * kPer + d] = q;
+                if (d % 8 == 0) scales[at * (HD / kGroup) + d / 8] = s;
+            }
+            const int next = c + kAhead * kThreads;
+            if (next < chunks) in[i] = __ldcs(x + next);
+        }
     }
 }
 
-int rows_entry(const char* what, const RowArgs& a, void (*kern)(RowArgs), cudaStream_t stream) {
-    const int64_t warps = (int64_t)a.n_rows * a.c.n_kv_head * 2 * (a.c.head_dim / kGroup);
-    const int64_t blocks = (warps + 7) / 8, most = 16ll * forge_sm_count();
-    kern<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(a);
-    return forge_check_launch(what);
+template <int HD>
+__global__ void __launch_bounds__(kThreads) k_kv4_read(const RowArgs a) {
+    constexpr int kPer = HD / 8;
+    const int64_t r = blockIdx.x;
+    const bool v = blockIdx.y;
+    const int chunks = a.c.n_kv_head * kPer;
+    const int p = a.pos[r];
+    if (p < 0) return;
+    const int64_t row = cache_row(a.c, a.seq ? a.seq[r] : (int)r, p, a.err);
+    const int64_t head_rows = a.c.table ? a.c.page_tokens : a.c.lmax;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(v ? a.c.v : a.c.k) + row * kPer;
+    const uint16_t* scales = (v ? a.c.vs : a.c.ks) + row * (HD / kGroup);
+    float4* out = reinterpret_cast<float4*>((v ? a.vo : a.ko) + r * a.ld);
+    for (int base = 0; base < chunks; base += kAhead * kThreads) {
+        uint32_t q[kAhead];
+        uint16_t s[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int c = base + i * kThreads + (int)threadIdx.x;
+            q[i] = 0;
+            s[i] = 0x7FC0;  // a row out of range reads as NaN
+            if (c < chunks && row >= 0) {
+                const int64_t at = (c / kPer) * head_rows;
+                q[i] = codes[at * kPer + c % kPer];
+                s[i] = scales[at * (HD / kGroup) + c % kPer / 8];
+            }
+        }
+        // a warp's 32 chunks in two stores of 512 contiguous bytes: lane l writes half l % 2 of chunk 16 j + l / 2
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (base + i * kThreads >= chunks) break;
+            const int lane = threadIdx.x & 31, first = base + i * kThreads + ((int)threadIdx.x & ~31);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int from = 16 * j + lane / 2;
+                const uint32_t w = __shfl_sync(0xffffffffu, q[i], from) >> (16 * (lane & 1));
+                const float f = bf16_bits_to_f32((uint16_t)__shfl_sync(0xffffffffu, (uint32_t)s[i], from));
+                F2 o[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)  // code in the low bits of 2^23, exact less 2^23 + 7
+                    o[k] = (F2(__uint_as_float((w >> (8 * k) & 15u) | 0x4B000000u), __uint_as_float((w >> (8 * k + 4) & 15u) | 0x4B000000u)) +
+                            F2(-8388615.0f, -8388615.0f)) * F2(f, f);
+                if (first + from < chunks) __stcs(out + 2 * first + 32 * j + lane, make_float4(o[0].x(), o[0].y(), o[1].x(), o[1].y()));
+            }
+        }
+    }
 }
 }  // namespace
 
@@ -126,7 +206,8 @@ extern "C" FORGE_API int forge_kv4_append(const ForgeKv4* cache, const uint16_t*
     uint32_t* err = forge_ops_err_word();
     if (!err) return forge_fail(-1, "forge_kv4_append: no device");
     RowArgs a{*cache, k, v, nullptr, nullptr, ld, seq, pos, n_rows, err};
-    return rows_entry("forge_kv4_append", a, k_kv4_append, (cudaStream_t)stream);
+    (cache->head_dim == 128 ? k_kv4_append<128> : k_kv4_append<64>)<<<dim3(n_rows, 2), kThreads, 0, (cudaStream_t)stream>>>(a);
+    return forge_check_launch("forge_kv4_append");
 }
 
 extern "C" FORGE_API int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos, int n_rows,
@@ -139,5 +220,6 @@ extern "C" FORGE_API int forge_kv4_read(const ForgeKv4* cache, const int32_t* se
     uint32_t* err = forge_ops_err_word();
     if (!err) return forge_fail(-1, "forge_kv4_read: no device");
     RowArgs a{*cache, nullptr, nullptr, k_out, v_out, ld, seq, pos, n_rows, err};
-    return rows_entry("forge_kv4_read", a, k_kv4_read, (cudaStream_t)stream);
+    (cache->head_dim == 128 ? k_kv4_read<128> : k_kv4_read<64>)<<<dim3(n_rows, 2), kThreads, 0, (cudaStream_t)stream>>>(a);
+    return forge_check_launch("forge_kv4_read");
 }

@@ -2,25 +2,31 @@
 //
 // out[h] = sum_j p_j v_j / sum_j p_j, p_j = exp(q_h . k_j / sqrt(hd)), with
 // k_jd = sk_jg (n_jd - 7) and v alike (n the 4-bit code, g the group of 64
-// dims). A KV head's keys are read once for up to 8 of its query heads, on
-// m16n8k16 fp16 tensor-core products with fp32 sums:
+// dims). A KV head's keys are read once for up to 4 of its query heads, on
+// m16n8k32 products of 8-bit integers with 32-bit sums, which are exact. The
+// codes are bytes after a mask (and a shift for odd dims of K); a factor in
+// fp32 becomes three base-256 digits in rows of the A operand: row r has digit
+// 2, 1 or 0 of head r % 4 for r < 4, r < 8, 8 <= r < 12.
 //
-//   S: A = q of 8 heads, rows 0-7 their fp16 heads and rows 8-15 what fp16
-//      left over (q is first scaled by a power of two so that its largest
-//      entry is near 2^15: the pair holds 22 bits), B = the codes of 8 keys.
-//      (word >> 8k) & 0x000F000F is the fp16 pair (n, n') 2^-24, a
-//      subnormal, & 0x00F000F0 sixteen times that, and one fp16 fma makes
-//      either (n - 7) 2^-9 (exact). Subnormals fed to the tensor cores as
-//      they are cost no fma, but a product is aligned by the exponent field,
-//      not by its leading bit, and cut off 2^-25 below that: scores came out
-//      8e-6 off. The key's scale multiplies each group's sum in fp32.
-//   O: A = the weights p_j sv_jg of 8 heads as fp16 and remainder, times a
-//      power of two that follows the largest scale seen, B = the codes of
-//      two keys per register (one byte permute per four dims), less 7 in
-//      the same way. A tile's product is added to O in fp32
-//      registers: no chain of tensor-core sums is longer than 4.
+//   S: q times a power of two as 24-bit integers, signed digits; -7 sum q is
+//      in the initial sum. A group's sum is multiplied by the key's scale in
+//      fp32.
+//   O: the weights p_j sv_jg of a tile as integers below 2^23, p relative to
+//      the tile's own maximum and sv to its largest scale: added to 2^23 their
+//      digits are the fp32's low bytes. ldmatrix transposes V's bytes, so that a
+//      register holds a byte of four keys; odd dims stay times 16 in theirs.
+//      One more product, with a constant 7, gives 7 times the sum of the
+//      weights, taken off exactly before the tile joins O in fp32.
 //
-// Work: the tiles of 64 keys of all (sequence, KV head, 8 query heads) form
+// A sum starts at 1.5 2^23 as an integer's bits, so its bits are the fp32
+// 12582912 + sum and need no conversion. (The same products in fp16, with q and
+// the weights as pairs of fp16, take twice the tensor time and three times the
+// unpacking: 389 us for 64 sequences of 4096 with 40 heads of 128, where this
+// takes 286, of which the cache's bytes need 218.) Bound: instructions, 0.44
+// of the issue slots' cycles with 2 warps a scheduler, and their latencies;
+// 3 warps a scheduler need 168 registers, which spill, and gain nothing.
+//
+// Work: the tiles of 64 keys of all (sequence, KV head, 4 query heads) form
 // one line, every pair's tiles behind a few units for what a pair costs by
 // itself, cut into one range per CTA, so a batch of very different lengths is
 // as even as one of equal ones. In a CTA each warp takes every fourth tile
@@ -28,7 +34,6 @@
 // range joins the four warps, and where a range ends inside a pair the last
 // CTA to arrive joins the CTAs that shared it, in the order of the keys.
 #include <cmath>
-#include <cuda_fp16.h>
 #include "common.cuh"
 #include "f32x2.cuh"
 #include "forge_internal.h"
@@ -43,7 +48,9 @@ constexpr int kStages = 2;         // tiles a warp has in flight
 constexpr int kCtasPerSm = 2;
 constexpr int kPairUnits = 4;      // what a pair costs beside its tiles, in tiles
 constexpr int kMinUnits = kWarps + kPairUnits;  // a range of one pair gives every warp a tile
-constexpr int kHeads = 8;          // query heads that share a pass over the keys
+constexpr int kJoin = kWarps / 2;  // sums of warps that shared memory holds at the end of a pair
+constexpr int kHeads = 4;          // query heads that share a pass over the keys
+constexpr int kMagic = 0x4B400000; // 1.5 2^23 as fp32
 
 template <int HD>
 struct Geo {
@@ -51,10 +58,11 @@ struct Geo {
     static constexpr int kCodes = kKeys * HD / 2, kScales = kKeys * kNG * 2;  // bytes of a tile, K or V
     static constexpr int kSlot = 2 * (kCodes + kScales);                      // K codes, V codes, K scales, V scales
     static constexpr int kRow = HD + 4;                                       // floats of a head in the join (no bank twice)
-    static constexpr int kOffQ = kWarps * kStages * kSlot;                    // [4 groups][32 lanes] A operands
-    static constexpr int kOffRed = kOffQ + 4 * kNG * 512;                     // [warp][8][kRow] sums of the warps
-    static constexpr int kOffMl = kOffRed + kWarps * kHeads * kRow * 4;       // [warp][8] m, then l
-    static constexpr int kOffBar = kOffMl + 2 * kWarps * kHeads * 4;
+    static constexpr int kOffQ = kWarps * kStages * kSlot;                    // [2 groups][32 lanes] A operands
+    static constexpr int kOffC = kOffQ + 2 * kNG * 512;                       // [groups][8] sums that the scores start from, kMagic
+    static constexpr int kOffRed = kOffC + kNG * 128 + 16;                    // [warp][kHeads][kRow] sums of warps
+    static constexpr int kOffMl = kOffRed + kJoin * kHeads * kRow * 4;        // [warp][kHeads] m, then l
+    static constexpr int kOffBar = kOffMl + 2 * kJoin * kHeads * 4;
     static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
 };
 
@@ -62,44 +70,69 @@ struct Kv4Args {
     ForgeKv4 c;
     const float* q;
     const int32_t *seq, *pos;
-    int B, H, G, nhb, ph;   // query heads, heads per KV head, blocks of 8 of them, (KV head, block) pairs
+    int B, H, G, nhb, ph;   // query heads, heads per KV head, blocks of kHeads of them, (KV head, block) pairs
     int cap;                // rows a sequence can hold
     float scale_log2;       // log2(e) / sqrt(hd)
     float* out;
     uint32_t* counters;     // [B][ph]
-    float* partial;         // [CTA][2][8][hd + 2]
+    float* partial;         // [CTA][2][kHeads][hd + 2]
     uint32_t* err;
 };
 
-// d = A B (+ c): m16n8k16, fp16 operands, fp32 sums.
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = A B + c: m16n8k32, 8-bit integers, 32-bit integer sums.
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, const int4& c) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
 }
-__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+__device__ __forceinline__ void mma_u8u8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, const int4& c) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
+}
+__device__ __forceinline__ int4 quad(const int (&d)[4]) { return make_int4(d[0], d[1], d[2], d[3]); }
+// The codes of even dims of a word (or of a byte of four keys), of odd ones times 16.
+__device__ __forceinline__ uint32_t even(uint32_t w) { return w & 0x0F0F0F0Fu; }
+__device__ __forceinline__ uint32_t odd16(uint32_t w) { return w & 0xF0F0F0F0u; }
+// Bytes of two words; a selector of 8 + b gives 0 where byte b is not negative.
+__device__ __forceinline__ uint32_t prmt(uint32_t x, uint32_t y, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t* w) { return prmt(prmt(w[0], w[1], 0x40), prmt(w[2], w[3], 0x40), 0x5410); }
+// Bytes of 32 rows of 16, transposed: r[k] has bytes g (k 0, 2) or 8 + g (k 1, 3) of rows 4 t .. 4 t + 3 (k 0, 1) or 16
+// more (k 2, 3). Lane l gives row l's address.
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[4], const uint8_t* row) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(row)));
+}
+// The scales of keys 4 r .. 4 r + 3, and those of keys 2 f, 2 f + 1 of them for a group.
+template <int NG>
+struct Scales {
+    uint32_t w[2 * NG];
+    __device__ __forceinline__ Scales(const uint8_t* base, int r) {
+        if constexpr (NG == 2) {
+            const uint4 v = reinterpret_cast<const uint4*>(base)[r];
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+            const uint2 v = reinterpret_cast<const uint2*>(base)[r];
+            w[0] = v.x; w[1] = v.y;
+        }
+    }
+    __device__ __forceinline__ F2 of(int f, int group) const {
+        if constexpr (NG == 1) return F2(bf16_lo_f32(w[f]), bf16_hi_f32(w[f]));
+        else return group ? F2(bf16_hi_f32(w[2 * f]), bf16_hi_f32(w[2 * f + 1])) : F2(bf16_lo_f32(w[2 * f]), bf16_lo_f32(w[2 * f + 1]));
+    }
+};
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p = 0;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\t@e mov.s32 %0, 1;\n\t}" : "+r"(p));
+    return p;
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-// x as fp16 and what that leaves, two values at once
-__device__ __forceinline__ void split_f16(F2 x, uint32_t& hi, uint32_t& lo) {
-    float r0, r1;  // hi - x
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x.y()), "f"(x.x()));
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}"
-        : "=f"(r0), "=f"(r1) : "r"(hi), "f"(x.x()), "f"(x.y()));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(-r1), "f"(-r0));
-}
-// The codes in bits 0-3 (lo) or 4-7 (hi) of both halves, less 7 and times
-// 2^-9, as an fp16 pair (exact).
-__device__ __forceinline__ uint32_t fma2_bits(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-__device__ __forceinline__ uint32_t code_lo(uint32_t w) { return fma2_bits(w & 0x000F000Fu, 0x78007800u, 0xA300A300u); }
-__device__ __forceinline__ uint32_t code_hi(uint32_t w) { return fma2_bits(w & 0x00F000F0u, 0x68006800u, 0xA300A300u); }
+__device__ __forceinline__ F2 float_bits(int x, int y) { return F2(__int_as_float(x), __int_as_float(y)); }
 
 // Tiles of sequence slot b; -1 when its position or sequence is out of range.
 __device__ __forceinline__ int tiles_of(const Kv4Args& a, int b) {
@@ -131,17 +164,23 @@ struct Place {
 template <int HD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Args a) {
     using X = Geo<HD>;
-    constexpr int NG = X::kNG, U = kKeys / 8, KK = kKeys / 16;
+    constexpr int NG = X::kNG, U = kKeys / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kStages * X::kSlot;
     uint4* qs = reinterpret_cast<uint4*>(smem + X::kOffQ);
+    int4* from = reinterpret_cast<int4*>(smem + X::kOffC);
     float* red = reinterpret_cast<float*>(smem + X::kOffRed);
     float* sm_m = reinterpret_cast<float*>(smem + X::kOffMl);
-    float* sm_l = sm_m + kWarps * kHeads;
+    float* sm_l = sm_m + kJoin * kHeads;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + X::kOffBar) + warp * kStages;
     __shared__ int s_last;
+    // this lane's rows of A: digit 2 or 1 of head h, and digit 0 or nothing
+    const int h = g & 3;
+    const float da = g < 4 ? 65536.f : 256.f, db = g < 4 ? 1.f : 0.f, off = -12582912.f * (da + db);
+    const uint32_t sel = g < 4 ? 0x4062 : 0xBB51;  // digits a of two words, then digits b
 
+    if (threadIdx.x == 0) from[8 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
@@ -222,12 +261,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         }
         const int s = n_in % kStages, key0 = in_j * kKeys;
         const int rows = min(kKeys, in_rows - key0);
-        uint8_t* dst = ring + s * X::kSlot + slot_off;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], rows * (HD + 4 * NG));
-        __syncwarp();
+        uint8_t* slot = ring + s * X::kSlot;
         if (!in_table) {
-            if (lane < 4) bulk_g2s_stream(dst, array + (in_row0 + key0) * unit, rows * unit, &full[s], l2_evict_first());
+            // (one thread and no loop: addresses in uniform registers, which a copy wants, four times cheaper than by lane)
+            if (elect_one()) {
+                const int64_t row = in_row0 + key0;
+                const uint64_t once = l2_evict_first();
+                mbar_arrive_expect_tx(&full[s], rows * (HD + 4 * NG));
+                bulk_g2s_stream(slot, a.c.k + row * (HD / 2), rows * (HD / 2), &full[s], once);
+                bulk_g2s_stream(slot + X::kCodes, a.c.v + row * (HD / 2), rows * (HD / 2), &full[s], once);
+                bulk_g2s_stream(slot + 2 * X::kCodes, a.c.ks + row * NG, rows * (NG * 2), &full[s], once);
+                bulk_g2s_stream(slot + 2 * X::kCodes + X::kScales, a.c.vs + row * NG, rows * (NG * 2), &full[s], once);
+            }
         } else {
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], rows * (HD + 4 * NG));
+            __syncwarp();
+            uint8_t* dst = slot + slot_off;
             const int pt = a.c.page_tokens, pg0 = key0 / pt + (lane >> 2);
             const int r0 = max(0, pg0 * pt - key0), r1 = min(rows, (pg0 + 1) * pt - key0);
             bool bad = false;
@@ -258,44 +307,58 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         const int kvh = at.pair / a.nhb, h0 = (at.pair % a.nhb) * kHeads, nh = min(kHeads, a.G - h0);
         const size_t qrow = (size_t)at.b * a.H + kvh * a.G + h0;
 
-        // q as A operands: head g, dims 64 i + 16 t + 8 w + {0..7}, fp16 pairs (d, d + 4) and (d + 1, d + 5)
-        // (in shared memory, one quarter from each warp: registers are short while the codes of V are unpacked)
+        // q as A operands, dims 64 i + 16 t + 8 w + {0, 2, 4, 6} and {1, 3, 5, 7} (in shared memory, word w of group i from
+        // warp 2 i + w), and the sums that they start from
         float fac;
         {
             float4 v[NG][4];
-            float mx = 0.f;
+            uint32_t mx = 0;  // largest |q| as bits
 #pragma unroll
             for (int i = 0; i < NG; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    v[i][j] = g < nh ? *reinterpret_cast<const float4*>(a.q + (qrow + g) * HD + 64 * i + 16 * t + 4 * j)
+                    v[i][j] = h < nh ? *reinterpret_cast<const float4*>(a.q + (qrow + h) * HD + 64 * i + 16 * t + 4 * j)
                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)), fmaxf(fabsf(v[i][j].z), fabsf(v[i][j].w))));
+                    mx = max(max(mx, __float_as_uint(fabsf(v[i][j].x))), __float_as_uint(fabsf(v[i][j].y)));
+                    mx = max(max(mx, __float_as_uint(fabsf(v[i][j].z))), __float_as_uint(fabsf(v[i][j].w)));
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // 2^e <= mx < 2^(e + 1); q 2^(14 - e) fits fp16
-            const int e = max(-110, min(120, (int)(__float_as_uint(mx) >> 23) - 127));
-            const F2 up(pow2i(14 - e), pow2i(14 - e));
-            fac = a.scale_log2 * 0x1p-5f * pow2i(e);  // 2^9 of the codes, 2^(e - 14) of q
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
+            const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
+            const float up = pow2i(23 - e);
+            fac = mx >= 0x7F800000u ? NAN : a.scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                // word warp / 2 of the 16 dims, dims 2 k, 2 k + 4 and 2 k + 1, 2 k + 5 of it, k = warp % 2
-                const float4 lo4 = warp & 2 ? v[i][2] : v[i][0], hi4 = warp & 2 ? v[i][3] : v[i][1];
-                const bool k = warp & 1;
-                uint4 r;
-                split_f16(F2(k ? lo4.z : lo4.x, k ? hi4.z : hi4.x) * up, r.x, r.y);
-                split_f16(F2(k ? lo4.w : lo4.y, k ? hi4.w : hi4.y) * up, r.z, r.w);
-                qs[(4 * i + warp) * 32 + lane] = r;
+                int sa = 0, sb = 0;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const float4 lo4 = v[i][2 * w], hi4 = v[i][2 * w + 1];
+                    const float x[8] = {lo4.x, lo4.z, hi4.x, hi4.z, lo4.y, lo4.w, hi4.y, hi4.w};  // even dims, odd dims
+                    uint32_t da[8], db[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
+                        da[k] = g < 4 ? (n1 - d1) >> 8 : d1;
+                        db[k] = g < 4 ? d0 : 0;
+                    }
+                    const uint4 r = make_uint4(low_bytes(da), low_bytes(db), low_bytes(da + 4), low_bytes(db + 4));
+                    if (warp == 2 * i + w) qs[(2 * i + w) * 32 + lane] = r;
+                    sa = __dp4a((int)r.z, 0x01010101, __dp4a((int)r.x, 0x01010101, sa));
+                    sb = __dp4a((int)r.w, 0x01010101, __dp4a((int)r.y, 0x01010101, sb));
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    sa += __shfl_xor_sync(0xffffffffu, sa, o);
+                    sb += __shfl_xor_sync(0xffffffffu, sb, o);
+                }
+                if (warp == 0 && t == 0) from[8 * i + g] = make_int4(kMagic - 7 * sa, kMagic - 7 * sa, kMagic - 7 * sb, kMagic - 7 * sb);
             }
         }
         __syncthreads();
 
-        // p_j = 2^(x_j - mref), mref = max x - 14 + e, e following the largest V scale: weights p_j sv_j stay below
-        // 2^14; l and o (times 2^9) are sums of those p
-        float m = -INFINITY, mref = -INFINITY;
-        F2 l(0.f, 0.f), o[NG][8];  // o[group][nibble]: dims 64 i + 16 t + n and + 8
-        int e_run = -88;
+        float m = -INFINITY;
+        F2 l(0.f, 0.f), o[NG][8];  // o[group][2 k + b]: dims 64 i + 16 k + 4 t + b and + 2, this lane's digits' part
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
@@ -311,105 +374,126 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
                 break;
             }
             const uint8_t* kc = ring + s * X::kSlot;
-            const uint8_t* vc = kc + X::kCodes;
-            const uint8_t* ks = vc + X::kCodes;
+            const uint8_t* ks = kc + 2 * X::kCodes;
+            const uint8_t* krow = kc + (4 * (g >> 1) + (g & 1)) * (HD / 2) + 8 * t;  // this lane's keys of B, and of V's transposition
+            const uint8_t* vrow = kc + X::kCodes + lane * (HD / 2);
             uint8_t* vs = const_cast<uint8_t*>(ks) + X::kScales;
             const int left = j + 1 < at.n ? kKeys : a.pos[at.b] + 1 - j * kKeys;  // keys of the tile
 
-            // ---- scores of keys 8 u + t and 8 u + 4 + t, head g, over fac
+            // ---- scores of keys 16 (u / 2) + 4 t + 2 (u % 2) + {0, 1}, head h, over fac
             F2 x[U];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                uint32_t qa[4][4];
+            for (int u0 = 0; u0 < U; u0 += 2) {
+                const Scales<NG> sk(ks, 2 * u0 + t);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint4 r = qs[(4 * i + k) * 32 + lane];
-                    qa[k][0] = r.x; qa[k][1] = r.y; qa[k][2] = r.z; qa[k][3] = r.w;
-                }
+                for (int i = 0; i < NG; ++i) {
+                    const uint4 q0 = qs[2 * i * 32 + lane], q1 = qs[(2 * i + 1) * 32 + lane];
+                    const int4 c0 = from[8 * i + g];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(kc + (8 * u + (g >> 1) + 4 * (g & 1)) * (HD / 2) + 32 * i + t * 8);
-                    const uint16_t s0 = *reinterpret_cast<const uint16_t*>(ks + ((8 * u + t) * NG + i) * 2);
-                    const uint16_t s1 = *reinterpret_cast<const uint16_t*>(ks + ((8 * u + 4 + t) * NG + i) * 2);
-                    float c[4];
-                    mma_f16_first(c, qa[0], code_lo(w.x), code_hi(w.x));
-                    mma_f16(c, qa[1], code_lo(w.x >> 8), code_hi(w.x >> 8));
-                    mma_f16(c, qa[2], code_lo(w.y), code_hi(w.y));
-                    mma_f16(c, qa[3], code_lo(w.y >> 8), code_hi(w.y >> 8));
-                    const F2 sum = F2(c[0], c[1]) + F2(c[2], c[3]), sc(bf16_bits_to_f32(s0), bf16_bits_to_f32(s1));
-                    x[u] = i ? fma2(sum, sc, x[u]) : sum * sc;
+                    for (int f = 0; f < 2; ++f) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(krow + (8 * u0 + 2 * f) * (HD / 2) + 32 * i);
+                        int c[4];
+                        mma_s8u8(c, q0, even(w.x), even(w.x >> 4), c0);
+                        mma_s8u8(c, q1, even(w.y), even(w.y >> 4), quad(c));
+                        // digit a times da + digit b times db; both offsets of 12582912 come off exactly with the first
+                        const F2 sum = fma2(float_bits(c[2], c[3]), F2(db, db), fma2(float_bits(c[0], c[1]), F2(da, da), F2(off, off)));
+                        x[u0 + f] = i ? fma2(sum, sk.of(f, i), x[u0 + f]) : sum * sk.of(f, i);
+                    }
                 }
             }
-            // ---- the tile's largest score and V scale; keys behind the last one count for nothing
+#pragma unroll
+            for (int u = 0; u < U; ++u)  // the other digits
+                x[u] = x[u] + F2(__shfl_xor_sync(0xffffffffu, x[u].x(), 16), __shfl_xor_sync(0xffffffffu, x[u].y(), 16));
+            // ---- the tile's largest score and V scales; keys behind the last one count for nothing
             if (left < kKeys) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    x[u] = F2(8 * u + t < left ? x[u].x() : -INFINITY, 8 * u + 4 + t < left ? x[u].y() : -INFINITY);
+                    {
+                    const int key = 8 * (u & ~1) + 2 * (u & 1) + 4 * t;
+                    x[u] = F2(key < left ? x[u].x() : -INFINITY, key + 1 < left ? x[u].y() : -INFINITY);
+                }
 #pragma unroll
                 for (int k = 0; k < kKeys * NG; k += 32)
                     if (k + lane >= left * NG) reinterpret_cast<uint16_t*>(vs)[k + lane] = 0;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
                 __syncwarp();
             }
-            uint32_t smax = 0;  // bf16 bits, two at a time
+            uint32_t smax = 0;  // bf16 bits: of group 0 and 1, or of even and odd keys
 #pragma unroll
             for (int k = 0; k < kKeys * NG / 2; k += 32)
                 if (k + lane < kKeys * NG / 2) smax = __vmaxu2(smax, reinterpret_cast<const uint32_t*>(vs)[k + lane] & 0x7FFF7FFFu);
-            smax = __reduce_max_sync(0xffffffffu, max(smax & 0xffffu, smax >> 16));
+            const uint32_t smax0 = __reduce_max_sync(0xffffffffu, smax & 0xffffu), smax1 = __reduce_max_sync(0xffffffffu, smax >> 16);
             float mx = fmaxf(x[0].x(), x[0].y());
 #pragma unroll
             for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            m = fmaxf(m, mx * fac);
-            e_run = max(e_run, min(129, (int)(smax >> 7) - 126));  // the same in all lanes
-            const float m_new = m - (float)(14 - e_run);
-            const float alpha = mref == -INFINITY ? 0.f : ex2(mref - m_new);
-            mref = m_new;
-            const float nref = m_new == -INFINITY ? 0.f : -m_new;
+            mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
+            // p = 2^(x - mx) <= 1
+            const float nmx = mx == -INFINITY ? 0.f : -mx;
             F2 ls;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const F2 y = fma2(x[u], F2(fac, fac), F2(nref, nref));
+                const F2 y = fma2(x[u], F2(fac, fac), F2(nmx, nmx));
                 x[u] = F2(ex2(y.x()), ex2(y.y()));
                 ls = u ? ls + x[u] : x[u];
             }
-            l = fma2(l, F2(alpha, alpha), ls);
+            // the tile's part of the sums, relative to the largest score so far
+            const float m_new = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : ex2(m - m_new);
+            const float beta = mx == -INFINITY ? 0.f : ex2(mx - m_new);
+            m = m_new;
+            l = fma2(l, F2(alpha, alpha), ls * F2(beta, beta));
 
             // ---- O += P V, group by group
+            const Scales<NG> sv[U / 2] = {{vs, t}, {vs, 4 + t}, {vs, 8 + t}, {vs, 12 + t}};
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                float c[8][4];
+                // weights p sv unit < 2^23: 2^23 + weight has them in its low bits. (rcp is off by an ulp, the same for the tile)
+                const uint32_t sx = NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0;
+                const float smx = fmaxf(bf16_bits_to_f32((uint16_t)sx), 0x1p-100f), unit = rcp(smx) * (8388608.f * 255.f / 256.f);
+                const float wa = beta * smx * (256.f / 255.f / 8388608.f) * da, wb = beta * smx * (256.f / 255.f / 8388608.f) * db;
+                const int4 magic = from[8 * NG];
+                uint4 pa[U / 4];
+                int c7[4];
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    uint32_t pa[4];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int key = 16 * kk + 8 * k + t;
-                        const uint16_t s0 = *reinterpret_cast<const uint16_t*>(vs + (key * NG + i) * 2);
-                        const uint16_t s1 = *reinterpret_cast<const uint16_t*>(vs + ((key + 4) * NG + i) * 2);
-                        split_f16(x[2 * kk + k] * F2(bf16_bits_to_f32(s0), bf16_bits_to_f32(s1)), pa[2 * k], pa[2 * k + 1]);
-                    }
-                    uint32_t r[4];  // word g of group i of keys 16 kk + t + {0, 4, 8, 12}
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        r[k] = *reinterpret_cast<const uint32_t*>(vc + (16 * kk + 4 * k + t) * (HD / 2) + 32 * i + 4 * g);
+                for (int kb = 0; kb < U / 4; ++kb) {
+                    uint32_t y[4];  // two digits of keys 32 kb + 16 (k / 2) + 4 t + 2 (k % 2) + {0, 1}
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        // byte k (nibbles 2 k and 2 k + 1) of two keys, one in either half
-                        const uint32_t p0 = __byte_perm(r[0], r[1], 0x4400 + 0x1111 * k);
-                        const uint32_t p1 = __byte_perm(r[2], r[3], 0x4400 + 0x1111 * k);
-                        if (kk == 0) {
-                            mma_f16_first(c[2 * k], pa, code_lo(p0), code_lo(p1));
-                            mma_f16_first(c[2 * k + 1], pa, code_hi(p0), code_hi(p1));
-                        } else {
-                            mma_f16(c[2 * k], pa, code_lo(p0), code_lo(p1));
-                            mma_f16(c[2 * k + 1], pa, code_hi(p0), code_hi(p1));
+                        const F2 n = fma2(x[4 * kb + k], sv[2 * kb + k / 2].of(k & 1, i) * F2(unit, unit), F2(8388608.f, 8388608.f));
+                        y[k] = prmt(__float_as_uint(n.x()), __float_as_uint(n.y()), sel);
+                    }
+                    pa[kb] = make_uint4(prmt(y[0], y[1], 0x5410), prmt(y[0], y[1], 0x7632), prmt(y[2], y[3], 0x5410), prmt(y[2], y[3], 0x7632));
+                    mma_u8u8(c7, pa[kb], 0x07070707u, 0x07070707u, kb ? quad(c7) : magic);
+                }
+                // odd dims are 16 times; digit a's 7s and offset come off exactly, digit b's to below a unit of the weights
+                const float a7 = __int_as_float(c7[0]), b7 = __int_as_float(c7[2]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // 16 bytes of the group's 32
+                    int c[4][4];
+#pragma unroll
+                    for (int kb = 0; kb < U / 4; ++kb) {
+                        uint32_t r[4];
+                        load_transposed(r, vrow + 32 * kb * (HD / 2) + 32 * i + 16 * j);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            mma_u8u8(c[2 * k], pa[kb], even(r[k]), even(r[k + 2]), kb ? quad(c[2 * k]) : magic);
+                            mma_u8u8(c[2 * k + 1], pa[kb], odd16(r[k]), odd16(r[k + 2]), kb ? quad(c[2 * k + 1]) : magic);
                         }
                     }
-                }
 #pragma unroll
-                for (int n = 0; n < 8; ++n)
-                    o[i][n] = fma2(o[i][n], F2(alpha, alpha), F2(c[n][0], c[n][1]) + F2(c[n][2], c[n][3]));
+                    for (int n = 0; n < 4; ++n) {
+                        const float ua = n & 1 ? wa * 0.0625f : wa, ub = n & 1 ? wb * 0.0625f : wb;
+                        const float ma = n & 1 ? fmaf(a7, -16.f, 15.f * 12582912.f) : -a7, mb = n & 1 ? fmaf(b7, -16.f, 15.f * 12582912.f) : -b7;
+                        const F2 na = float_bits(c[n][0], c[n][1]) + F2(ma, ma);
+                        const F2 join = fma2(o[i][4 * j + n], F2(alpha, alpha), F2(mb * ub, mb * ub));
+                        o[i][4 * j + n] = fma2(na, F2(ua, ua), fma2(float_bits(c[n][2], c[n][3]), F2(ub, ub), join));
+                    }
+                }
+                // (a scale that is no number has no digits)
+                if (sx >= 0x7F80u)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) o[i][n] = F2(NAN, NAN);
             }
             if (poison >> s & 1) l = F2(NAN, NAN);
             ++n_out;
@@ -418,29 +502,47 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         }
         if (dead) l = F2(NAN, NAN);
 
-        // ---- join the warps: their sums with their (mref, l)
+        // ---- join the warps: the upper half's sums into the lower half's, then those over the CTA
         float lw = l.x() + l.y();
         lw += __shfl_xor_sync(0xffffffffu, lw, 1);
         lw += __shfl_xor_sync(0xffffffffu, lw, 2);
-        if (t == 0) {
-            sm_m[warp * kHeads + g] = mref;
-            sm_l[warp * kHeads + g] = lw;
-        }
-        if (g < nh) {
-            float* dst = red + (warp * kHeads + g) * X::kRow + 16 * t;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                o[i][n] = o[i][n] + F2(__shfl_xor_sync(0xffffffffu, o[i][n].x(), 16), __shfl_xor_sync(0xffffffffu, o[i][n].y(), 16));
+        const int slot = warp % kJoin * kHeads + h;
+        float* mine = red + slot * X::kRow + 4 * t;
+        if (warp >= kJoin && g < nh) {
 #pragma unroll
             for (int i = 0; i < NG; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int n = 0; n < 8; n += 2)
+                    *reinterpret_cast<float4*>(mine + 64 * i + 8 * n) = make_float4(o[i][n].x(), o[i][n + 1].x(), o[i][n].y(), o[i][n + 1].y());
+            if (t == 0) {
+                sm_m[slot] = m;
+                sm_l[slot] = lw;
+            }
+        }
+        __syncthreads();
+        const float mo = sm_m[slot], lo = sm_l[slot];
+        __syncwarp();
+        if (warp < kJoin && g < nh) {
+            const float mj = fmaxf(m, mo);
+            const float f = m == -INFINITY ? 0.f : ex2(m - mj), fo = mo == -INFINITY ? 0.f : ex2(mo - mj);
+            if (t == 0) {
+                sm_m[slot] = mj;
+                sm_l[slot] = isnan(lo) || isnan(lw) ? NAN : fmaf(lw, f, lo * fo);
+            }
 #pragma unroll
-                    for (int n = 0; n < 8; n += 4) {
-                        float4 v;
-                        v.x = k ? o[i][n].y() : o[i][n].x();
-                        v.y = k ? o[i][n + 1].y() : o[i][n + 1].x();
-                        v.z = k ? o[i][n + 2].y() : o[i][n + 2].x();
-                        v.w = k ? o[i][n + 3].y() : o[i][n + 3].x();
-                        *reinterpret_cast<float4*>(dst + 64 * i + 8 * k + n) = v;
-                    }
+            for (int i = 0; i < NG; ++i)
+#pragma unroll
+                for (int n = 0; n < 8; n += 2) {
+                    float4 v = *reinterpret_cast<const float4*>(mine + 64 * i + 8 * n);
+                    v.x = fmaf(o[i][n].x(), f, v.x * fo); v.y = fmaf(o[i][n + 1].x(), f, v.y * fo);
+                    v.z = fmaf(o[i][n].y(), f, v.z * fo); v.w = fmaf(o[i][n + 1].y(), f, v.w * fo);
+                    *reinterpret_cast<float4*>(mine + 64 * i + 8 * n) = v;
+                }
         }
         __syncthreads();
         const int unit0 = at.base + kPairUnits, cfirst = unit0 / per, clast = (unit0 + at.n - 1) / per;
@@ -449,17 +551,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             const int h = idx / (HD / 4), d = idx % (HD / 4) * 4;
             float mj = -INFINITY, lj = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mj = fmaxf(mj, sm_m[w * kHeads + h]);
+            for (int w = 0; w < kJoin; ++w) mj = fmaxf(mj, sm_m[w * kHeads + h]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < kJoin; ++w) {
                 const float mw = sm_m[w * kHeads + h], lv = sm_l[w * kHeads + h];
                 const float f = mw == -INFINITY ? 0.f : ex2(mw - mj);
                 lj = isnan(lv) ? lv : fmaf(lv, f, lj);
                 const float4 r = *reinterpret_cast<const float4*>(red + (w * kHeads + h) * X::kRow + d);
                 v.x = fmaf(r.x, f, v.x); v.y = fmaf(r.y, f, v.y); v.z = fmaf(r.z, f, v.z); v.w = fmaf(r.w, f, v.w);
             }
-            const float il = 512.f / lj;
+            const float il = 1.f / lj;
             v.x *= il; v.y *= il; v.z *= il; v.w *= il;
             if (cfirst == clast) {
                 *reinterpret_cast<float4*>(a.out + (qrow + h) * HD + d) = v;
@@ -488,10 +590,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         __syncthreads();
         if (!s_last) continue;
         const int nc = clast - cfirst + 1;
-        for (int h = warp; h < nh; h += kWarps) {
+        for (int hh = warp; hh < nh; hh += kWarps) {
             // contribution c: the pair starts in the first CTA's range and before every other's
             auto slot = [&](int c) {
-                return a.partial + ((size_t)(cfirst + c) * 2 + (c == 0)) * kHeads * (HD + 2) + h * (HD + 2);
+                return a.partial + ((size_t)(cfirst + c) * 2 + (c == 0)) * kHeads * (HD + 2) + hh * (HD + 2);
             };
             float mm = -INFINITY;
             for (int c = lane; c < nc; c += 32) mm = fmaxf(mm, __ldcg(slot(c) + HD));
@@ -528,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             }
 #pragma unroll
             for (int e = 0; e < E / 2; ++e)
-                reinterpret_cast<float2*>(a.out + (qrow + h) * HD)[32 * e + lane] = make_float2(acc[2 * e] / sum, acc[2 * e + 1] / sum);
+                reinterpret_cast<float2*>(a.out + (qrow + hh) * HD)[32 * e + lane] = make_float2(acc[2 * e] / sum, acc[2 * e + 1] / sum);
         }
     }
 }

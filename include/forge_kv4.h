@@ -61,8 +61,8 @@ int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos
  * over positions 0..pos[b] of sequence seq[b] (seq NULL: sequence b), query
  * head h reading KV head h / (H / n_kv_head). q and out [B][H * head_dim]
  * fp32, 16-byte aligned; H a multiple of n_kv_head; scores, softmax and sums
- * in fp32 (the products on the tensor cores with q and the probabilities as
- * pairs of fp16, about 22 bits). pos[b] < 0: an empty sequence, its output is
+ * in fp32 (the products on the tensor cores in integers, exactly: q and the
+ * weights of 64 keys rounded to 23 bits of their largest). pos[b] < 0: an empty sequence, its output is
  * zeros (a padded batch). A position beyond the cache, or a page outside the
  * pool, sets the error word and makes the sequence's output NaN.
  * workspace: forge_flash_decode_kv4_workspace_bytes(...) bytes, 16-byte

@@ -187,10 +187,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
     }
 
     // ---- the line's length; sequences without tiles are answered here
+    const int n0 = lane < a.B ? tiles_of(a, lane) : 0;
     int total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int b = b0 + lane;
-        const int n = b < a.B ? tiles_of(a, b) : 0;
+        const int n = b0 == 0 ? n0 : b < a.B ? tiles_of(a, b) : 0;
         if (warp == 0) {
             unsigned none = __ballot_sync(0xffffffffu, b < a.B && n <= 0 && b % (int)gridDim.x == (int)blockIdx.x);
             for (; none; none &= none - 1) {
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
     Place at{0, 0, 0, 0};
     for (int b0 = 0;; b0 += 32) {  // at.base: first unit of slot b0
         const int b = b0 + lane;
-        const int n = b < a.B ? max(0, tiles_of(a, b)) : 0, un = n ? n + kPairUnits : 0;
+        const int n = max(0, b0 == 0 ? n0 : b < a.B ? tiles_of(a, b) : 0), un = n ? n + kPairUnits : 0;
         int inc = un;
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -296,14 +297,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         in_j += kWarps;
         ++n_in;
     };
+    // q of a pair (dims 64 i + 16 t .. + 15 of head h), loaded before what it can be loaded before
+    float4 v[NG][4];
+    auto load_q = [&](const Place& p) {
+        const int h0 = (p.pair % a.nhb) * kHeads;
+        const float* q = a.q + ((size_t)p.b * a.H + p.pair / a.nhb * a.G + h0 + h) * HD + 16 * t;
+        const bool mine = p.lo(start) < p.hi(end) && h < a.G - h0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[i][j] = mine ? *reinterpret_cast<const float4*>(q + 64 * i + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    load_q(at);
     for (int s = 0; s < kStages; ++s) issue();
 
     int n_out = 0;
     bool dead = false;  // a wait ran out: nothing more is read
-    for (; at.base < end; at.next(a)) {
+    for (Place following = at; at.base < end; at = following) {
         // ---- one pair: tiles [j0, j1)
         const int j0 = at.lo(start), j1 = at.hi(end);
-        if (j0 >= j1) continue;
+        if (j0 >= j1) break;  // (the range ends before the pair's first tile)
         const int kvh = at.pair / a.nhb, h0 = (at.pair % a.nhb) * kHeads, nh = min(kHeads, a.G - h0);
         const size_t qrow = (size_t)at.b * a.H + kvh * a.G + h0;
 
@@ -311,14 +325,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         // warp 2 i + w), and the sums that they start from
         float fac;
         {
-            float4 v[NG][4];
             uint32_t mx = 0;  // largest |q| as bits
 #pragma unroll
             for (int i = 0; i < NG; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    v[i][j] = h < nh ? *reinterpret_cast<const float4*>(a.q + (qrow + h) * HD + 64 * i + 16 * t + 4 * j)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f);
                     mx = max(max(mx, __float_as_uint(fabsf(v[i][j].x))), __float_as_uint(fabsf(v[i][j].y)));
                     mx = max(max(mx, __float_as_uint(fabsf(v[i][j].z))), __float_as_uint(fabsf(v[i][j].w)));
                 }
@@ -501,6 +512,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             issue();
         }
         if (dead) l = F2(NAN, NAN);
+        following.next(a);
+        load_q(following);
 
         // ---- join the warps: the upper half's sums into the lower half's, then those over the CTA
         float lw = l.x() + l.y();
@@ -595,38 +608,38 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
             auto slot = [&](int c) {
                 return a.partial + ((size_t)(cfirst + c) * 2 + (c == 0)) * kHeads * (HD + 2) + hh * (HD + 2);
             };
+            constexpr int E = HD / 32;
+            float2 p[8][E / 2];
+            auto fetch = [&](int c) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e)
+                        if (c + k < nc) p[k][e] = __ldcg(reinterpret_cast<const float2*>(slot(c + k)) + 32 * e + lane);
+            };
+            fetch(0);
             float mm = -INFINITY;
             for (int c = lane; c < nc; c += 32) mm = fmaxf(mm, __ldcg(slot(c) + HD));
             for (int d = 16; d; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-            constexpr int E = HD / 32;
-            float acc[E] = {}, sum = 0.f;
-            for (int c0 = 0; c0 < nc; c0 += 32) {
-                float wl = 0.f;
-                if (c0 + lane < nc) {
-                    const float mc = __ldcg(slot(c0 + lane) + HD), lc = __ldcg(slot(c0 + lane) + HD + 1);
+            float acc[E] = {}, sum = 0.f, wl = 0.f;
+            for (int c = 0; c < nc; c += 8) {
+                if (c % 32 == 0 && c + lane < nc) {
+                    const float mc = __ldcg(slot(c + lane) + HD), lc = __ldcg(slot(c + lane) + HD + 1);
                     wl = mc == -INFINITY && !isnan(lc) ? 0.f : lc * ex2(mc - mm);
                 }
-                const int cn = min(32, nc - c0);
-                for (int c = 0; c < cn; c += 8) {
-                    float2 v[8][E / 2];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < 8; ++k) {
+                    const float w = __shfl_sync(0xffffffffu, wl, (c + k) & 31);
+                    if (c + k < nc) {
+                        sum += w;
 #pragma unroll
-                        for (int e = 0; e < E / 2; ++e)
-                            if (c + k < cn) v[k][e] = __ldcg(reinterpret_cast<const float2*>(slot(c0 + c + k)) + 32 * e + lane);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float w = __shfl_sync(0xffffffffu, wl, (c + k) & 31);
-                        if (c + k < cn) {
-                            sum += w;
-#pragma unroll
-                            for (int e = 0; e < E / 2; ++e) {
-                                acc[2 * e] = w == 0.f ? acc[2 * e] : fmaf(w, v[k][e].x, acc[2 * e]);
-                                acc[2 * e + 1] = w == 0.f ? acc[2 * e + 1] : fmaf(w, v[k][e].y, acc[2 * e + 1]);
-                            }
+                        for (int e = 0; e < E / 2; ++e) {
+                            acc[2 * e] = w == 0.f ? acc[2 * e] : fmaf(w, p[k][e].x, acc[2 * e]);
+                            acc[2 * e + 1] = w == 0.f ? acc[2 * e + 1] : fmaf(w, p[k][e].y, acc[2 * e + 1]);
                         }
                     }
                 }
+                fetch(c + 8);
             }
 #pragma unroll
             for (int e = 0; e < E / 2; ++e)

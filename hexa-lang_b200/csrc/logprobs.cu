@@ -18,8 +18,8 @@
 // over the 8 warps of the ceil(top / 8)-th largest that lanes hold), and it
 // is raised in the same way after 4, 16, 64 groups; a group's maximum, which
 // the softmax needs, is compared with it, and the few vectors that reach it
-// go to a list. At the end the listed vectors are read again, and one warp
-// cuts their keys to at most 64 by bisection and orders those by counting.
+// go to a list. At the end the keys of the list's vectors that reach it are
+// ordered by counting, each thread those above its own.
 // Rows whose list overflows (rising logits) are collected once more, with the
 // list cut to the best whenever it is full.
 //
@@ -40,9 +40,8 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kVecs = 4;             // vectors of a thread in a group, in flight together
 constexpr int kMaxTop = FORGE_LOGPROBS_MAX_TOP;
-constexpr int kList = 512;           // candidate vectors (kFew threads' of one batch fit)
-constexpr int kKeys = 256;           // keys that one warp selects from (8 a lane; a cluster's 8 times 32)
-constexpr int kFew = 64;             // keys ordered by counting
+constexpr int kList = 512;           // candidate vectors
+constexpr int kKeys = 256;           // keys that are ordered by counting (a cluster's 8 times 32)
 constexpr int kCtasPerSm = 4;
 // Logits below kFloor count as kFloor and c is at least kLeast log2 e: such
 // logits have no weight beside any above kLeast, and no infinity arises. Rows
@@ -158,8 +157,9 @@ struct Stats {
 };
 
 struct Shared {
-    int list[kList];                        // candidate vectors
-    uint64_t keys[kKeys], few[kFew];
+    uint4 vec[kList];                       // candidate vectors
+    int list[kList];                        // and which they are
+    alignas(16) uint64_t keys[kKeys];
     uint64_t best[kMaxTop];                 // largest first; 0 where there are fewer
     uint64_t gather[kKeys];                 // the cluster's best, in its first CTA
     uint64_t edge[16], bound[kWarps];
@@ -201,55 +201,22 @@ __device__ uint64_t bisect(Shared& sh, int want, int most, F count) {
 }
 
 // The largest `top` of the n keys in sh.keys (fewer if there are fewer) into
-// sh.best, in order, by the first warp alone: at most kFew by bisection from
-// `floor`, which at least `top` keys reach, then by counting.
-__device__ __forceinline__ void select(Shared& sh, int n, int top, uint64_t floor) {
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        uint64_t k[kKeys / 32], hi = 0;
+// sh.best, in order: a thread counts the keys above its own.
+__device__ __forceinline__ void select(Shared& sh, int n, int top) {
+    static_assert(kKeys == kThreads, "a key a thread");
+    const uint64_t k = (int)threadIdx.x < n ? sh.keys[threadIdx.x] : 0;
+    if (threadIdx.x < kMaxTop) sh.best[threadIdx.x] = 0;
+    if ((int)threadIdx.x >= n && (int)threadIdx.x < ((n + 7) & ~7)) sh.keys[threadIdx.x] = 0;
+    __syncthreads();
+    if (k) {
+        int above = 0;
+        for (int i = 0; i < n; i += 8)
 #pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) {
-            k[i] = i * 32 + lane < n ? sh.keys[i * 32 + lane] : 0;
-            hi = max(hi, k[i]);
-        }
-        sh.best[lane] = 0;
-        uint64_t lo = 1;  // (0 is no key)
-        if (n > kFew) {
-            lo = max(lo, floor);
-            const uint32_t top32 = __reduce_max_sync(0xffffffffu, (uint32_t)(hi >> 32));
-            hi = (uint64_t)top32 << 32 | 0xFFFFFFFFu;
-            while (lo < hi) {
-                const uint64_t mid = lo + (hi - lo) / 2 + 1;
-                int c = 0;
-#pragma unroll
-                for (int i = 0; i < kKeys / 32; ++i) c += k[i] >= mid;
-                c = __reduce_add_sync(0xffffffffu, c);
-                if (c < top) {
-                    hi = mid - 1;
-                } else {
-                    lo = mid;
-                    if (c <= kFew) break;
-                }
+            for (int j = 0; j < 8; j += 2) {
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(sh.keys + i + j);
+                above += (x.x > k) + (x.y > k);
             }
-        }
-        int few = 0;
-#pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) {
-            const bool in = k[i] >= lo;
-            const unsigned who = __ballot_sync(0xffffffffu, in);
-            if (in) sh.few[few + __popc(who & ((1u << lane) - 1))] = k[i];
-            few += __popc(who);
-        }
-        __syncwarp();
-        const uint64_t k0 = lane < few ? sh.few[lane] : 0, k1 = lane + 32 < few ? sh.few[lane + 32] : 0;
-        int b0 = 0, b1 = 0;
-        for (int i = 0; i < few; ++i) {
-            const uint64_t x = sh.few[i];
-            b0 += x > k0;
-            b1 += x > k1;
-        }
-        if (k0 && b0 < top) sh.best[b0] = k0;
-        if (k1 && b1 < top) sh.best[b1] = k1;
+        if (above < top) sh.best[above] = k;
     }
     __syncthreads();
 }
@@ -257,7 +224,7 @@ __device__ __forceinline__ void select(Shared& sh, int n, int top, uint64_t floo
 // The best of the listed vectors, the keys in sh.edge and those already in
 // sh.best, into sh.best; floor: a key that at least `top` of them reach (or 1).
 template <typename T>
-__device__ __noinline__ void settle(Shared& sh, const T* z, int head, int listed, int top, uint64_t floor) {
+__device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, uint64_t floor) {
     using V = Vec<T>;
     uint64_t own = 0;
     if (threadIdx.x < kMaxTop) own = sh.best[threadIdx.x];
@@ -267,7 +234,7 @@ __device__ __noinline__ void settle(Shared& sh, const T* z, int head, int listed
 #pragma unroll 1
         for (int i = threadIdx.x; i < listed; i += kThreads) {
             const int first = head + sh.list[i] * V::kN;
-            const uint4 v = *reinterpret_cast<const uint4*>(z + first);
+            const uint4 v = sh.vec[i];
 #pragma unroll
             for (int j = 0; j < V::kN / 2; ++j) {
                 f(key_of(V::raw(v, j).x(), first + 2 * j));
@@ -294,7 +261,7 @@ __device__ __noinline__ void settle(Shared& sh, const T* z, int head, int listed
         n = gather(floor);
     }
     if (threadIdx.x < 16) sh.edge[threadIdx.x] = 0;
-    select(sh, n, top, floor);
+    select(sh, n, top);
 }
 
 // The best of vectors [v0, v1) and the keys in sh.edge into sh.best, for rows
@@ -307,14 +274,16 @@ __device__ __noinline__ void collect(Shared& sh, const T* z, int head, int v0, i
     for (int base = v0; base < v1; base += kThreads) {
         const int i = base + (int)threadIdx.x;
         uint64_t key = 0;
+        uint4 v = make_uint4(0, 0, 0, 0);
         if (i < v1) {
+            v = *reinterpret_cast<const uint4*>(z + head + (int64_t)i * V::kN);
             typename V::Max m;
-            m.add(*reinterpret_cast<const uint4*>(z + head + (int64_t)i * V::kN));
+            m.add(v);
             key = key_of(m.get(), i);
         }
         bool in = key && key >= thr;
         if (listed + __syncthreads_count(in) > kList) {
-            settle(sh, z, head, listed, top, thr ? sh.best[top - 1] : 1);
+            settle<T>(sh, head, listed, top, thr ? sh.best[top - 1] : 1);
             listed = 0;
             if (const uint64_t last = sh.best[top - 1]) thr = key_of(value_of(last), max(0, index_of(last) - head) / V::kN);
             in = key && key >= thr;
@@ -322,11 +291,15 @@ __device__ __noinline__ void collect(Shared& sh, const T* z, int head, int v0, i
         }
         if (threadIdx.x == 0) sh.n = listed;
         __syncthreads();
-        if (in) sh.list[atomicAdd(&sh.n, 1)] = i;
+        if (in) {
+            const int at = atomicAdd(&sh.n, 1);
+            sh.list[at] = i;
+            sh.vec[at] = v;
+        }
         __syncthreads();
         listed = sh.n;
     }
-    settle(sh, z, head, listed, top, thr ? sh.best[top - 1] : 1);
+    settle<T>(sh, head, listed, top, thr ? sh.best[top - 1] : 1);
 }
 
 // exp(z - m) and (z - m) exp(z - m) over a row by the calling CTA, for
@@ -371,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
     // the CTA's vectors [v0, v1) of the row, cut at 16-byte boundaries of memory
     const int head = min(a.V, (int)(((16 - ((uintptr_t)z & 15)) & 15) / sizeof(T)));
     const int vecs = (a.V - head) / V::kN;
-    const int v0 = (int)((int64_t)vecs * part / cluster), v1 = (int)((int64_t)vecs * (part + 1) / cluster);
+    const int v0 = (int)((unsigned)vecs * part / cluster), v1 = (int)((unsigned)vecs * (part + 1) / cluster);
     const uint4* zv = reinterpret_cast<const uint4*>(z + head);
     uint4 v[kVecs];
     auto load = [&](int k, int base) {  // vector k of this thread in the group at base
@@ -397,26 +370,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
     float m = -INFINITY, c = kLeast * kLog2e;
     F2 s(0.f, 0.f), t(0.f, 0.f);
     int rank = 0;
-    // ---- the row's ends outside the vectors (an element each for a few threads), and the token's own vector
-    if (part == 0) {
-        const int tail = head + vecs * V::kN;
-        const int i = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;
-        if (i < a.V) {
-            const float x = V::one(z + i);
-            if (top) sh.edge[threadIdx.x] = key_of(x, i);
-            if (has) rank += i < y ? !(fmaxf(x, -INFINITY) < fy) : x > fy;
-            m = fmaxf(x, -INFINITY);
-            c = fmaxf(m, kLeast) * kLog2e;
-            const float w = fmaf(x < kFloor ? kFloor : x, kLog2e, -c), e = ex2(w);
-            s = F2(e, 0.f);
-            t = F2(e * w, 0.f);
-        }
-        if (has && yv >= 0 && threadIdx.x < V::kN && yv < vecs) {
-            const int j = head + yv * V::kN + (int)threadIdx.x;
-            rank += j < y && fmaxf(V::one(z + j), -INFINITY) == fy;
-        }
-    }
-    if (top) __syncthreads();
+    // the row's ends outside the vectors (an element each for a few threads), and the token's own vector
+    const int tail = head + vecs * V::kN;
+    const int edge = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;
+    const bool has_edge = part == 0 && edge < a.V;
+    const float ze = has_edge ? V::one(z + edge) : 0.f;
+    const bool beside = part == 0 && has && threadIdx.x < V::kN && yv >= 0 && yv < vecs;
+    const float zb = beside ? V::one(z + head + yv * V::kN + (int)threadIdx.x) : 0.f;
 
     // vectors that may hold one of the best reach (thr, thr_v): a larger maximum than thr, or that and an index up to thr_v
     float thr = -INFINITY;
@@ -470,7 +430,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
                     const float vm1 = x.get();
                     if (i < v1 && (vm1 > thr || (first && vm1 == thr && i <= thr_v))) {
                         const int at = atomicAdd(&sh.n, 1);
-                        if (at < kList) sh.list[at] = i;
+                        if (at < kList) {
+                            sh.list[at] = i;
+                            sh.vec[at] = v[k];
+                        }
                     }
                 }
             }
@@ -498,6 +461,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         }
         rank += cnt.get();
     }
+    if (has_edge) {
+        if (top) sh.edge[threadIdx.x] = key_of(ze, edge);
+        if (has) rank += edge < y ? !(fmaxf(ze, -INFINITY) < fy) : ze > fy;
+        m = fmaxf(m, ze);
+        const float n = fmaxf(m, kLeast) * kLog2e, d = c - n, f = ex2(d);
+        const float w = fmaf(ze < kFloor ? kFloor : ze, kLog2e, -n), e = ex2(w);
+        t = fma2(s, F2(d, d), t) * F2(f, f) + F2(e * w, 0.f);
+        s = s * F2(f, f) + F2(e, 0.f);
+        c = n;
+    }
+    if (beside) rank += head + yv * V::kN + (int)threadIdx.x < y && fmaxf(zb, -INFINITY) == fy;
     // ---- the block's sums and order
     Stats r{c, s.x() + s.y(), t.x() + t.y()};
 #pragma unroll
@@ -520,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         const int listed = sh.n;
         __syncthreads();
         if (listed > kList) collect(sh, z, head, v0, v1, top);
-        else settle(sh, z, head, listed, top, thr_v == INT_MAX ? (uint64_t)1 : (uint64_t)ordered(thr) << 32);
+        else settle<T>(sh, head, listed, top, thr_v == INT_MAX ? (uint64_t)1 : (uint64_t)ordered(thr) << 32);
     }
     // (the first warp alone: fewer instructions for the other rows' CTAs to wait behind)
     if (warp == 0) {
@@ -550,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         if (top) {
             if ((int)threadIdx.x < cluster * top) sh.keys[threadIdx.x] = sh.gather[threadIdx.x];
             __syncthreads();
-            select(sh, cluster * top, top, 1);
+            select(sh, cluster * top, top);
         }
         if (warp == 0) {
             r = sh.gstat[0];
@@ -576,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         if ((int)threadIdx.x < top) {
             const int id = index_of(sh.best[threadIdx.x]);
             if (a.ids) a.ids[(int64_t)row * top + threadIdx.x] = id;
-            if (a.tops) a.tops[(int64_t)row * top + threadIdx.x] = log_p(V::one(z + id));
+            if (a.tops) a.tops[(int64_t)row * top + threadIdx.x] = log_p(value_of(sh.best[threadIdx.x]));
         }
     };
     const bool odd = (m < kLeast || m > -kHuge) && !isinf(m);

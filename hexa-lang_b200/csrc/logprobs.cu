@@ -44,9 +44,10 @@ constexpr int kList = 512;           // candidate vectors
 constexpr int kKeys = 256;           // keys that are ordered by counting (a cluster's 8 times 32)
 constexpr int kCtasPerSm = 4;
 // Logits below kFloor count as kFloor and c is at least kLeast log2 e: such
-// logits have no weight beside any above kLeast, and no infinity arises. Rows
-// with a maximum below kLeast (or above -kHuge) are summed again, slowly.
-constexpr float kFloor = -1e30f, kLeast = -1e29f, kHuge = -2e38f;
+// logits have no weight beside any above kLeast, and no infinity arises. c is
+// m log2 e rounded, 2^-24 of it beside the exponent of the maximum itself: rows
+// with a maximum beyond +-kFar, where that is 0.09, are summed again, slowly.
+constexpr float kFloor = -1e30f, kLeast = -1e29f, kFar = 1e6f;
 constexpr int kMaxCluster = 8;
 
 struct LogprobArgs {
@@ -303,7 +304,7 @@ __device__ __noinline__ void collect(Shared& sh, const T* z, int head, int v0, i
 }
 
 // exp(z - m) and (z - m) exp(z - m) over a row by the calling CTA, for
-// maxima so far out that log2 e times them is no fp32 number.
+// maxima so far out that log2 e times them is too coarse, or no fp32 number.
 template <typename T>
 __device__ __noinline__ void slow_sums(Shared& sh, const T* z, int n, float m, float* s_out, float* t_out) {
     float s = 0.f, t = 0.f;
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
             if (a.tops) a.tops[(int64_t)row * top + threadIdx.x] = log_p(value_of(sh.best[threadIdx.x]));
         }
     };
-    const bool odd = (m < kLeast || m > -kHuge) && !isinf(m);
+    const bool odd = fabsf(m) > kFar && !isinf(m);
     if (!__syncthreads_or(warp == 0 && odd)) {
         if (warp == 0) answer(false);
         return;

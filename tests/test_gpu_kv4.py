@@ -4,8 +4,8 @@ forge_flash_decode_kv4) against plain float64 code.
 Codes and scales are exact: they equal forge_q4_quantize_bf16's with group 64
 and a restatement of the rule. The attention's tolerance follows from its
 arithmetic. With u = 2^-23 (one step of a truncating fp32 sum), a score of hd
-products is off by at most ds = (hd + 4) u sum|q k| / sqrt(hd) (hd sums, and
-q's fp16 pair, 2^-22, counted twice for its two products); a probability
+products is off by at most ds = (hd + 4) u sum|q k| / sqrt(hd) (hd sums, and q
+rounded to 2^-23 of its largest channel, below 4 times the mean); a probability
 relative to the largest by 2 ds + 8 u max|s| (the exponent's argument and its
 exp2); a sum over n keys in tiles by (64 + n / 64) u; so the output by
 vmax (4 ds + (16 smax + 2 (64 + n / 64) + 16) u), vmax the largest |v|."""

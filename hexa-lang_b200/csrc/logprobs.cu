@@ -14,9 +14,9 @@
 // equal and the lowest index wins. Candidates are whole 16-byte vectors,
 // ordered by (largest logit, lowest index) in the same way: when `top`
 // vectors reach a threshold, every vector that does not has `top` entries
-// before its own. The first group of vectors sets the threshold (the smallest
-// over the 8 warps of the ceil(top / 8)-th largest that lanes hold), and it
-// is raised in the same way after 4, 16, 64 groups; a group's maximum, which
+// before its own. The first group of vectors sets the threshold (the
+// top-th largest of what remains of each warp's largest few), and it is raised
+// in the same way after 4, 16, 64 groups; a group's maximum, which
 // the softmax needs, is compared with it, and the few vectors that reach it
 // go to a list. At the end the keys of the list's vectors that reach it are
 // ordered by counting, each thread those above its own.
@@ -163,12 +163,19 @@ struct Shared {
     alignas(16) uint64_t keys[kKeys];
     uint64_t best[kMaxTop];                 // largest first; 0 where there are fewer
     uint64_t gather[kKeys];                 // the cluster's best, in its first CTA
-    uint64_t edge[16], bound[kWarps];
+    uint64_t edge[16], bound[kMaxTop];
     Stats stat[kWarps], gstat[kMaxCluster];
     float max[kWarps], gmax[kMaxCluster];
     int rank[kWarps], grank[kMaxCluster], part[kWarps];
     int n;
 };
+
+// The warp's largest number.
+__device__ __forceinline__ uint64_t warp_max(uint64_t x) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
+    return (uint64_t)hi << 32 | lo;
+}
 
 // Sum over the block.
 __device__ __forceinline__ int block_sum(Shared& sh, int c) {
@@ -230,7 +237,7 @@ __device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, u
     uint64_t own = 0;
     if (threadIdx.x < kMaxTop) own = sh.best[threadIdx.x];
     else if (threadIdx.x < kMaxTop + 16) own = sh.edge[threadIdx.x - kMaxTop];
-    auto each = [&](auto f) {
+    auto each = [&](float least, auto f) {  // the keys of logits not below `least`
         if (own) f(own);
 #pragma unroll 1
         for (int i = threadIdx.x; i < listed; i += kThreads) {
@@ -238,8 +245,9 @@ __device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, u
             const uint4 v = sh.vec[i];
 #pragma unroll
             for (int j = 0; j < V::kN / 2; ++j) {
-                f(key_of(V::raw(v, j).x(), first + 2 * j));
-                f(key_of(V::raw(v, j).y(), first + 2 * j + 1));
+                const F2 x = V::raw(v, j);
+                if (!(x.x() < least)) f(key_of(x.x(), first + 2 * j));
+                if (!(x.y() < least)) f(key_of(x.y(), first + 2 * j + 1));
             }
         }
     };
@@ -247,7 +255,7 @@ __device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, u
         __syncthreads();
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
-        each([&](uint64_t key) {
+        each(cut > 1 ? value_of(cut) : -INFINITY, [&](uint64_t key) {
             if (key >= cut) {
                 const int at = atomicAdd(&sh.n, 1);
                 if (at < kKeys) sh.keys[at] = key;
@@ -258,7 +266,7 @@ __device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, u
     };
     int n = gather(floor);
     if (n > kKeys) {  // equal or rising logits
-        floor = bisect(sh, top, kKeys, [&](uint64_t x) { int c = 0; each([&](uint64_t key) { c += key >= x; }); return c; });
+        floor = bisect(sh, top, kKeys, [&](uint64_t x) { int c = 0; each(-INFINITY, [&](uint64_t key) { c += key >= x; }); return c; });
         n = gather(floor);
     }
     if (threadIdx.x < 16) sh.edge[threadIdx.x] = 0;
@@ -382,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
     // vectors that may hold one of the best reach (thr, thr_v): a larger maximum than thr, or that and an index up to thr_v
     float thr = -INFINITY;
     int thr_v = INT_MAX;
+    const int rounds = min(kMaxTop / kWarps, (top + 4 + kWarps - 1) / kWarps);  // at least `top` numbers, a few more if there is room
     int group = 0;
     for (int base = v0; base < v1; base += kGroup, ++group) {
         typename V::Max vm;
@@ -391,9 +400,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         if (top) {
             const bool first = group == 0;
             if (first || group == 4 || group == 16 || group == 64) {
-                // the ceil(top / 8)-th largest of each warp's lanes: of the vectors of the first group by (maximum, index),
-                // later of all so far by value; 0 where fewer lanes have a vector (no threshold)
-                uint64_t mine = 0, nth = 0;
+                // the largest few of each warp's lanes: of the vectors of the first group by (maximum, index), later of all
+                // so far by value; 0 where fewer lanes have a vector
+                uint64_t mine = 0, nth;
                 if (first) {
 #pragma unroll
                     for (int k = 0; k < kVecs; ++k) {
@@ -405,18 +414,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
                 } else {
                     mine = key_of(fmaxf(m, gm), (int)threadIdx.x);
                 }
-                for (int r = 0; r < (top + kWarps - 1) / kWarps; ++r) {
-                    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
-                    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == hi ? (uint32_t)mine : 0u);
-                    nth = (uint64_t)hi << 32 | lo;
+                __syncthreads();
+                for (int r = 0; r < rounds; ++r) {
+                    nth = warp_max(mine);
                     if (mine == nth) mine = 0;
+                    if (lane == 0) sh.bound[r * kWarps + warp] = nth;
                 }
                 __syncthreads();
-                if (lane == 0) sh.bound[warp] = nth;
-                __syncthreads();
-                uint64_t b = sh.bound[0];
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) b = min(b, sh.bound[w]);
+                // the top-th largest of those: the last of `top` maxima, or what is left without the smallest
+                uint64_t b = lane < rounds * kWarps ? sh.bound[lane] : 0;
+                const int n = __popc(__ballot_sync(0xffffffffu, b != 0));
+                if (n < top) {
+                    b = 0;  // no threshold
+                } else if (top <= n - top) {
+                    for (int r = 1; r < top; ++r)
+                        if (b == warp_max(b)) b = 0;
+                    b = warp_max(b);
+                } else {
+                    b = b ? ~b : 0;
+                    for (int r = 0; r < n - top; ++r)
+                        if (b == warp_max(b)) b = 0;
+                    b = ~warp_max(b);
+                }
                 if (b && (first || value_of(b) > thr)) {
                     thr = value_of(b);
                     thr_v = first ? index_of(b) : -1;

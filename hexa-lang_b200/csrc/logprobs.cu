@@ -11,15 +11,15 @@
 //
 // Top alternatives: entries are ordered by a 64-bit key, the logit as an
 // ordered integer above the complement of its index, so that no two are
-// equal and the lowest index wins. Candidates are whole 16-byte vectors,
-// ordered by (largest logit, lowest index) in the same way: when `top`
-// vectors reach a threshold, every vector that does not has `top` entries
-// before its own. The first group of vectors sets the threshold (the
-// top-th largest of what remains of each warp's largest few), and it is raised
-// in the same way after 4, 16, 64 groups; a group's maximum, which
-// the softmax needs, is compared with it, and the few vectors that reach it
-// go to a list. At the end the keys of the list's vectors that reach it are
-// ordered by counting, each thread those above its own.
+// equal and the lowest index wins. Candidates are the vectors of a thread in a
+// group, ordered by their largest logit: when `top` candidates reach a
+// threshold, every one that does not has `top` entries before its own. The
+// first group sets the threshold (the top-th largest of what is left of each
+// warp's largest few), and it is raised in the same way in groups 2, 8, 32; a
+// group's maximum, which the softmax needs, is compared with it, and the few
+// that reach it go to a list. At the end their logits are read again and the
+// keys of those that reach it ordered by counting, each thread those above its
+// own.
 // Rows whose list overflows (rising logits) are collected once more, with the
 // list cut to the best whenever it is full.
 //
@@ -40,7 +40,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kVecs = 4;             // vectors of a thread in a group, in flight together
 constexpr int kMaxTop = FORGE_LOGPROBS_MAX_TOP;
-constexpr int kList = 512;           // candidate vectors
+constexpr int kList = 512;           // candidates (all threads' of the first group fit)
 constexpr int kKeys = 256;           // keys that are ordered by counting (a cluster's 8 times 32)
 constexpr int kCtasPerSm = 4;
 // Logits below kFloor count as kFloor and c is at least kLeast log2 e: such
@@ -158,8 +158,7 @@ struct Stats {
 };
 
 struct Shared {
-    uint4 vec[kList];                       // candidate vectors
-    int list[kList];                        // and which they are
+    int list[kList];                        // candidates: a thread's vectors of a group, by the first of them
     alignas(16) uint64_t keys[kKeys];
     uint64_t best[kMaxTop];                 // largest first; 0 where there are fewer
     uint64_t gather[kKeys];                 // the cluster's best, in its first CTA
@@ -175,6 +174,38 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t x) {
     const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32));
     const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
     return (uint64_t)hi << 32 | lo;
+}
+
+__device__ __forceinline__ uint32_t warp_max(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
+
+// A number that at least `top` threads' numbers reach, close below the top-th
+// largest: the top-th of the `rounds` largest of each warp. 0 where that finds
+// fewer that are not 0.
+template <typename N>
+__device__ __forceinline__ N top_th(Shared& sh, N x, int rounds, int top) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto drop = [&](N& x) {  // the warp's largest, taken out once
+        const N big = warp_max(x);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, x == big)) - 1) x = 0;
+        return big;
+    };
+    N* bound = reinterpret_cast<N*>(sh.bound);
+    __syncthreads();
+    for (int r = 0; r < rounds; ++r) {
+        const N big = drop(x);
+        if (lane == 0) bound[r * kWarps + warp] = big;
+    }
+    __syncthreads();
+    N b = lane < rounds * kWarps ? bound[lane] : 0;
+    const int n = __popc(__ballot_sync(0xffffffffu, b != 0));
+    if (n < top) return 0;
+    if (top <= n - top) {
+        for (int r = 1; r < top; ++r) drop(b);
+        return warp_max(b);
+    }
+    b = b ? ~b : 0;
+    for (int r = 0; r < n - top; ++r) drop(b);
+    return ~warp_max(b);
 }
 
 // Sum over the block.
@@ -229,10 +260,11 @@ __device__ __forceinline__ void select(Shared& sh, int n, int top) {
     __syncthreads();
 }
 
-// The best of the listed vectors, the keys in sh.edge and those already in
-// sh.best, into sh.best; floor: a key that at least `top` of them reach (or 1).
-template <typename T>
-__device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, uint64_t floor) {
+// The best of the listed candidates, the keys in sh.edge and those already in
+// sh.best, into sh.best; a candidate is `per` vectors kThreads apart, those
+// behind v1 left out; floor: a key that at least `top` of them reach (or 1).
+template <typename T, int per>
+__device__ __forceinline__ void settle(Shared& sh, const T* z, int head, int v1, int listed, int top, uint64_t floor) {
     using V = Vec<T>;
     uint64_t own = 0;
     if (threadIdx.x < kMaxTop) own = sh.best[threadIdx.x];
@@ -240,9 +272,10 @@ __device__ __noinline__ void settle(Shared& sh, int head, int listed, int top, u
     auto each = [&](float least, auto f) {  // the keys of logits not below `least`
         if (own) f(own);
 #pragma unroll 1
-        for (int i = threadIdx.x; i < listed; i += kThreads) {
-            const int first = head + sh.list[i] * V::kN;
-            const uint4 v = sh.vec[i];
+        for (int i = threadIdx.x; i < listed * per; i += kThreads) {
+            const int at = sh.list[i / per] + i % per * kThreads, first = head + at * V::kN;
+            if (at >= v1) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(z + first);
 #pragma unroll
             for (int j = 0; j < V::kN / 2; ++j) {
                 const F2 x = V::raw(v, j);
@@ -283,16 +316,14 @@ __device__ __noinline__ void collect(Shared& sh, const T* z, int head, int v0, i
     for (int base = v0; base < v1; base += kThreads) {
         const int i = base + (int)threadIdx.x;
         uint64_t key = 0;
-        uint4 v = make_uint4(0, 0, 0, 0);
         if (i < v1) {
-            v = *reinterpret_cast<const uint4*>(z + head + (int64_t)i * V::kN);
             typename V::Max m;
-            m.add(v);
+            m.add(*reinterpret_cast<const uint4*>(z + head + (int64_t)i * V::kN));
             key = key_of(m.get(), i);
         }
         bool in = key && key >= thr;
         if (listed + __syncthreads_count(in) > kList) {
-            settle<T>(sh, head, listed, top, thr ? sh.best[top - 1] : 1);
+            settle<T, 1>(sh, z, head, v1, listed, top, thr ? sh.best[top - 1] : 1);
             listed = 0;
             if (const uint64_t last = sh.best[top - 1]) thr = key_of(value_of(last), max(0, index_of(last) - head) / V::kN);
             in = key && key >= thr;
@@ -300,15 +331,11 @@ __device__ __noinline__ void collect(Shared& sh, const T* z, int head, int v0, i
         }
         if (threadIdx.x == 0) sh.n = listed;
         __syncthreads();
-        if (in) {
-            const int at = atomicAdd(&sh.n, 1);
-            sh.list[at] = i;
-            sh.vec[at] = v;
-        }
+        if (in) sh.list[atomicAdd(&sh.n, 1)] = i;
         __syncthreads();
         listed = sh.n;
     }
-    settle<T>(sh, head, listed, top, thr ? sh.best[top - 1] : 1);
+    settle<T, 1>(sh, z, head, v1, listed, top, thr ? sh.best[top - 1] : 1);
 }
 
 // exp(z - m) and (z - m) exp(z - m) over a row by the calling CTA, for
@@ -387,9 +414,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
     const bool beside = part == 0 && has && threadIdx.x < V::kN && yv >= 0 && yv < vecs;
     const float zb = beside ? V::one(z + head + yv * V::kN + (int)threadIdx.x) : 0.f;
 
-    // vectors that may hold one of the best reach (thr, thr_v): a larger maximum than thr, or that and an index up to thr_v
+    // A group's vectors of a thread are a candidate where their largest logit reaches the threshold: in the first group
+    // by (logit, index), later by being larger than thr.
     float thr = -INFINITY;
-    int thr_v = INT_MAX;
+    bool have = false;
     const int rounds = min(kMaxTop / kWarps, (top + 4 + kWarps - 1) / kWarps);  // at least `top` numbers, a few more if there is room
     int group = 0;
     for (int base = v0; base < v1; base += kGroup, ++group) {
@@ -398,64 +426,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         for (int k = 0; k < kVecs; ++k) vm.add(v[k]);
         const float gm = vm.get();
         if (top) {
-            const bool first = group == 0;
-            if (first || group == 4 || group == 16 || group == 64) {
-                // the largest few of each warp's lanes: of the vectors of the first group by (maximum, index), later of all
-                // so far by value; 0 where fewer lanes have a vector
-                uint64_t mine = 0, nth;
-                if (first) {
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) {
-                        const int i = base + k * kThreads + (int)threadIdx.x;
-                        typename V::Max x;
-                        x.add(v[k]);
-                        if (i < v1) mine = max(mine, key_of(x.get(), i));
-                    }
-                } else {
-                    mine = key_of(fmaxf(m, gm), (int)threadIdx.x);
-                }
-                __syncthreads();
-                for (int r = 0; r < rounds; ++r) {
-                    nth = warp_max(mine);
-                    if (mine == nth) mine = 0;
-                    if (lane == 0) sh.bound[r * kWarps + warp] = nth;
-                }
-                __syncthreads();
-                // the top-th largest of those: the last of `top` maxima, or what is left without the smallest
-                uint64_t b = lane < rounds * kWarps ? sh.bound[lane] : 0;
-                const int n = __popc(__ballot_sync(0xffffffffu, b != 0));
-                if (n < top) {
-                    b = 0;  // no threshold
-                } else if (top <= n - top) {
-                    for (int r = 1; r < top; ++r)
-                        if (b == warp_max(b)) b = 0;
-                    b = warp_max(b);
-                } else {
-                    b = b ? ~b : 0;
-                    for (int r = 0; r < n - top; ++r)
-                        if (b == warp_max(b)) b = 0;
-                    b = ~warp_max(b);
-                }
-                if (b && (first || value_of(b) > thr)) {
-                    thr = value_of(b);
-                    thr_v = first ? index_of(b) : -1;
-                }
-            }
-            if (gm > thr || (first && gm == thr)) {
+            bool in;
+            if (group == 0) {
+                uint64_t key = 0;  // 0: no vector
 #pragma unroll
                 for (int k = 0; k < kVecs; ++k) {
                     const int i = base + k * kThreads + (int)threadIdx.x;
                     typename V::Max x;
                     x.add(v[k]);
-                    const float vm1 = x.get();
-                    if (i < v1 && (vm1 > thr || (first && vm1 == thr && i <= thr_v))) {
-                        const int at = atomicAdd(&sh.n, 1);
-                        if (at < kList) {
-                            sh.list[at] = i;
-                            sh.vec[at] = v[k];
-                        }
-                    }
+                    if (i < v1) key = max(key, key_of(x.get(), i));
                 }
+                const uint64_t b = top_th<uint64_t>(sh, key, rounds, top);
+                have = b != 0;
+                if (have) thr = value_of(b);
+                in = key && key >= b;
+            } else {
+                in = gm > thr;
+                if (group == 2 || group == 8 || group == 32) {  // (those that reach it may be this group's: not yet without equality)
+                    thr = fmaxf(thr, value_of((uint64_t)top_th<uint32_t>(sh, ordered(fmaxf(m, gm)), rounds, top) << 32));
+                    in = in && gm >= thr;
+                }
+            }
+            if (in) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kList) sh.list[at] = base + (int)threadIdx.x;
             }
         }
         if (gm > m) {
@@ -514,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_logprobs(const Logprob
         const int listed = sh.n;
         __syncthreads();
         if (listed > kList) collect(sh, z, head, v0, v1, top);
-        else settle<T>(sh, head, listed, top, thr_v == INT_MAX ? (uint64_t)1 : (uint64_t)ordered(thr) << 32);
+        else settle<T, kVecs>(sh, z, head, v1, listed, top, have ? (uint64_t)ordered(thr) << 32 : (uint64_t)1);
     }
     // (the first warp alone: fewer instructions for the other rows' CTAs to wait behind)
     if (warp == 0) {

@@ -229,6 +229,31 @@ def test_rising_and_flat_bf16_rows(forge, cuda, R):
         assert abs(got["entropy"][r] - got["entropy"][r % 3]) <= 4 * lp.T * (1 + got["entropy"][r])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 8, 20, 32])
+def test_best_logits_in_one_stretch(forge, cuda, dtype, top):
+    """All the best entries in one stretch of 1024 vectors of the row, one or two to a vector, whichever stretch it is:
+    where a threshold is taken from them, the last of them equals it."""
+    import torch
+    per = 4 if dtype == "f32" else 8
+    V, R = 1024 * per * 10 + 5, 11
+    z = torch.rand(R, V, generator=torch.Generator().manual_seed(6))
+    for r in range(R):
+        for j in range(top):
+            at = min(V - 1, (1024 * r + (j * 37) % 256 + 256 * (j % 4)) * per + (j * 5) % per)
+            z[r, at] = 4 + j / 16
+    z = z.to(torch.float32 if dtype == "f32" else torch.bfloat16)
+    pad = (-V) % 8  # every row starts on 16 bytes
+    d = torch.zeros(R, V + pad, dtype=z.dtype, device=cuda)
+    d[:, :V] = z
+    many = d.repeat(60, 1)[:, :V]  # enough rows for a CTA each
+    tok = [(97 * r) % V for r in range(60 * R)]
+    got = lp.call(forge, torch, many, tok, top)
+    lp.check(z.double().numpy(), tok[:R], top, {k: v[:R] for k, v in got.items()})
+    for r in range(R, 60 * R):
+        assert np.array_equal(got["ids"][r], got["ids"][r % R])
+
+
 def test_logits_far_from_zero(forge, cuda):
     """Maxima far from 0, where a logit times log2 e has no room for a fraction, or is no fp32 number."""
     import torch

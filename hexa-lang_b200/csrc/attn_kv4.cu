@@ -21,10 +21,13 @@
 // A sum starts at 1.5 2^23 as an integer's bits, so its bits are the fp32
 // 12582912 + sum and need no conversion. (The same products in fp16, with q and
 // the weights as pairs of fp16, take twice the tensor time and three times the
-// unpacking: 389 us for 64 sequences of 4096 with 40 heads of 128, where this
-// takes 286, of which the cache's bytes need 218.) Bound: instructions, 0.44
-// of the issue slots' cycles with 2 warps a scheduler, and their latencies;
-// 3 warps a scheduler need 168 registers, which spill, and gain nothing.
+// unpacking: 379 us for 64 sequences of 4096 with 40 heads of 128, where this
+// takes 265 back to back, 5.4 TB/s, of which the cache's bytes need 218.)
+// Bound there: the issue and latencies of about 840 instructions a tile with 2
+// warps a scheduler (0.49 of the issue slots) and shared memory (0.61 of its
+// wavefronts, half of them ldmatrix, whose rows 64 bytes apart share banks);
+// 3 warps a scheduler have 168 registers, spill, and come to the same. Short
+// contexts are a chain of latencies: 10 us for one sequence of 2048.
 //
 // Work: the tiles of 64 keys of all (sequence, KV head, 4 query heads) form
 // one line, every pair's tiles behind a few units for what a pair costs by

@@ -19,13 +19,17 @@
 // group's maximum, which the softmax needs, is compared with it, and the few
 // that reach it go to a list. At the end their logits are read again and the
 // keys of those that reach it ordered by counting, each thread those above its
-// own.
-// Rows whose list overflows (rising logits) are collected once more, with the
-// list cut to the best whenever it is full.
+// own. Rows whose list overflows (rising logits) are collected once
+// more, with the list cut to the best whenever it is full.
 //
-// What bounds it: HBM for many rows. For few rows
-// a row is shared by a cluster of CTAs that join through distributed shared
-// memory: no workspace and no second launch.
+// What bounds it: 2048 rows of 50257 in bf16 with 20 alternatives take 68 us
+// (3.0 TB/s, the bytes alone 31), by instructions: 0.68 of the issue slots,
+// about 80 for 8 logits of a thread without alternatives (48 us) and 45 more
+// with them. For few rows a row is shared by a cluster of CTAs that join
+// through distributed shared memory, without a workspace or a second launch:
+// one row of 32000 takes 6 us, launch and latencies. CTAs that stay and load
+// their next row during the end of one took 104 us: rows then start and end
+// together, and their ends no longer hide behind other rows' streams.
 #include <climits>
 #include <cmath>
 #include <cooperative_groups.h>

@@ -33,6 +33,12 @@
 // only when a score exceeds it by more than 2^8, so O in TMEM is rarely
 // rescaled.
 //
+// What bounds it: 8 prompts of 4096 with 32 heads take 0.99 ms in a burst
+// (1.1 PFLOP/s) and 1.15 under the power cap; the tensor cores' operands from
+// shared memory take as long as the products (1280 of about 1660 cycles for 64
+// keys of both tiles). 16 ragged prompts up to 4096, 32 heads on 8: 240 us
+// (0.88 PFLOP/s, clock 1.63 GHz). Short prompts: the longest item's steps.
+//
 // A sequence may end inside a key block. Keys behind it are masked by the
 // causal mask already; their V rows are zeroed in shared memory before the
 // product (0 times what the next sequence holds there might be NaN). Rows

@@ -306,9 +306,10 @@ int forge_sample(const float* logits, int64_t ld, int batch, int vocab, double t
  * Each output may be NULL; tokens may be NULL without logprob and rank. A
  * logit of -inf has no probability; a row of nothing else (or with a NaN, or
  * +inf) has NaN log probabilities and entropy, and is still ranked (NaN as
- * -inf). Sums in fp32, in an order fixed by the shape: the same bits every
- * time. Asynchronous on stream; no workspace. The reference computes none of
- * these (its sampler keeps the probabilities, self/ml/gpu_sampler.hexa:89-140). */
+ * -inf). Sums in fp32, in an order fixed by the shape and the rows' alignment:
+ * the same bits every time. Asynchronous on stream; no workspace. The
+ * reference computes none of these (its sampler keeps the probabilities,
+ * self/ml/gpu_sampler.hexa:89-140). */
 #define FORGE_LOGITS_F32  0
 #define FORGE_LOGITS_BF16 1
 #define FORGE_LOGPROBS_MAX_TOP 32

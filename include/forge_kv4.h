@@ -21,7 +21,10 @@
  * Every entry is asynchronous on `stream` and returns 0 or a FORGE_* code. A
  * position, sequence or page id that only the device can see to be out of
  * range sets the error word that forge_ops_check() reads; such a row is not
- * written by append and reads as NaN. */
+ * written by append and reads as NaN. Every call may be captured into a graph
+ * (the descriptor is copied, the arrays it names are not); the first call of
+ * any per-op entry on a device allocates that word and comes before a
+ * capture. */
 #ifndef FORGE_KV4_H
 #define FORGE_KV4_H
 #include <stdint.h>
@@ -62,9 +65,10 @@ int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos
  * head h reading KV head h / (H / n_kv_head). q and out [B][H * head_dim]
  * fp32, 16-byte aligned; H a multiple of n_kv_head; scores, softmax and sums
  * in fp32 (the products on the tensor cores in integers, exactly: q and the
- * weights of 64 keys rounded to 23 bits of their largest). pos[b] < 0: an empty sequence, its output is
- * zeros (a padded batch). A position beyond the cache, or a page outside the
- * pool, sets the error word and makes the sequence's output NaN.
+ * weights of 64 keys rounded to 23 bits of their largest). pos[b] < 0: an
+ * empty sequence, its output is zeros (a padded batch). A position beyond the
+ * cache, or a page outside the pool, sets the error word and makes the
+ * sequence's output NaN.
  * workspace: forge_flash_decode_kv4_workspace_bytes(...) bytes, 16-byte
  * aligned, zeroed once before first use (every call leaves its counters at
  * zero); calls that may overlap on the GPU, captured graphs among them, need

@@ -2,11 +2,9 @@
 //
 // out[h] = sum_j p_j v_j / sum_j p_j, p_j = exp(q_h . k_j / sqrt(hd)), with
 // k_jd = sk_jg (n_jd - 7) and v alike (n the 4-bit code, g the group of 64
-// dims). A KV head's keys are read once for up to 4 of its query heads, on
-// m16n8k32 products of 8-bit integers with 32-bit sums, which are exact. The
-// codes are bytes after a mask (and a shift for odd dims of K); a factor in
-// fp32 becomes three base-256 digits in rows of the A operand: row r has digit
-// 2, 1 or 0 of head r % 4 for r < 4, r < 8, 8 <= r < 12.
+// dims). The products are m16n8k32 ones of 8-bit integers with 32-bit sums,
+// which are exact. The codes are bytes after a mask (and a shift for odd dims of
+// K); a factor in fp32 becomes three base-256 digits.
 //
 //   S: q times a power of two as 24-bit integers, signed digits; -7 sum q is
 //      in the initial sum. A group's sum is multiplied by the key's scale in
@@ -19,23 +17,31 @@
 //      weights, taken off exactly before the tile joins O in fp32.
 //
 // A sum starts at 1.5 2^23 as an integer's bits, so its bits are the fp32
-// 12582912 + sum and need no conversion. (The same products in fp16, with q and
-// the weights as pairs of fp16, take twice the tensor time and three times the
-// unpacking: 379 us for 64 sequences of 4096 with 40 heads of 128, where this
-// takes 265 back to back, 5.4 TB/s, of which the cache's bytes need 218.)
-// Bound there: the issue and latencies of about 840 instructions a tile with 2
-// warps a scheduler (0.49 of the issue slots) and shared memory (0.61 of its
-// wavefronts, half of them ldmatrix, whose rows 64 bytes apart share banks);
-// 3 warps a scheduler have 168 registers, spill, and come to the same. Short
-// contexts are a chain of latencies: 10 us for one sequence of 2048.
+// 12582912 + sum and need no conversion.
 //
-// Work: the tiles of 64 keys of all (sequence, KV head, 4 query heads) form
+// Two forms, for how many query heads read a KV head. Up to 2: keys and dims
+// are the 16 rows of A and the digits of both heads 6 of the 8 columns, so a lane
+// has half of a tile's scores, exponentials and sums of the other form, about
+// 560 instructions for 64 keys of 128 dims, and 165 registers let 3 CTAs share
+// an SM. 3 and more: 4 heads' digits are 12 of the 16 rows, keys and dims the 8
+// columns, about 840 instructions, fewer than two passes of the first form, and
+// the keys are read once for the 4. Measured, 64 sequences of 4096 with 40 heads
+// of 128, each reading its own KV head (1.43 GB; 218 us at the rate of a copy):
+// 220 us in the first form, 6.5 TB/s, bound by HBM; 265 in the second, bound by
+// issue and latencies (0.49 of the issue slots with 2 warps a scheduler; 3 would
+// have 168 registers and spill) and shared-memory banks (0.61 of the wavefronts:
+// ldmatrix's rows 64 bytes apart share them). The same products in fp16, q and
+// weights as pairs of fp16, took 379. Short contexts are a chain of latencies:
+// 10 us for one sequence of 2048.
+//
+// Work: the tiles of 64 keys of all (sequence, KV head, heads of a pass) form
 // one line, every pair's tiles behind a few units for what a pair costs by
 // itself, cut into one range per CTA, so a batch of very different lengths is
 // as even as one of equal ones. In a CTA each warp takes every fourth tile
 // with a ring of bulk copies and a softmax of its own; a pair's end in the
 // range joins the four warps, and where a range ends inside a pair the last
 // CTA to arrive joins the CTAs that shared it, in the order of the keys.
+#include <algorithm>
 #include <cmath>
 #include "common.cuh"
 #include "f32x2.cuh"
@@ -48,11 +54,11 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 64;          // keys per tile
 constexpr int kStages = 2;         // tiles a warp has in flight
-constexpr int kCtasPerSm = 2;
-constexpr int kPairUnits = 4;      // what a pair costs beside its tiles, in tiles
-constexpr int kMinUnits = kWarps + kPairUnits;  // a range of one pair gives every warp a tile
+constexpr int kCtasMany = 2, kCtasFew = 3;  // CTAs per SM
+constexpr int kPairUnits = 6;      // what a pair costs beside its tiles, in tiles (4: 29.3 us for 32 ragged sequences, 6: 28.3)
+constexpr int kMinUnits = 2 * kWarps;  // least range of a CTA
 constexpr int kJoin = kWarps / 2;  // sums of warps that shared memory holds at the end of a pair
-constexpr int kHeads = 4;          // query heads that share a pass over the keys
+constexpr int kHeadsMany = 4, kHeadsFew = 2;  // query heads that share a pass over the keys
 constexpr int kMagic = 0x4B400000; // 1.5 2^23 as fp32
 
 template <int HD>
@@ -60,25 +66,18 @@ struct Geo {
     static constexpr int kNG = HD / FORGE_KV4_GROUP;
     static constexpr int kCodes = kKeys * HD / 2, kScales = kKeys * kNG * 2;  // bytes of a tile, K or V
     static constexpr int kSlot = 2 * (kCodes + kScales);                      // K codes, V codes, K scales, V scales
-    static constexpr int kRow = HD + 4;                                       // floats of a head in the join (no bank twice)
-    static constexpr int kOffQ = kWarps * kStages * kSlot;                    // [2 groups][32 lanes] A operands
-    static constexpr int kOffC = kOffQ + 2 * kNG * 512;                       // [groups][8] sums that the scores start from, kMagic
-    static constexpr int kOffRed = kOffC + kNG * 128 + 16;                    // [warp][kHeads][kRow] sums of warps
-    static constexpr int kOffMl = kOffRed + kJoin * kHeads * kRow * 4;        // [warp][kHeads] m, then l
-    static constexpr int kOffBar = kOffMl + 2 * kJoin * kHeads * 4;
-    static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
 };
 
 struct Kv4Args {
     ForgeKv4 c;
     const float* q;
     const int32_t *seq, *pos;
-    int B, H, G, nhb, ph;   // query heads, heads per KV head, blocks of kHeads of them, (KV head, block) pairs
+    int B, H, G, nhb, ph;   // query heads, heads per KV head, blocks of them that share a pass, (KV head, block) pairs
     int cap;                // rows a sequence can hold
     float scale_log2;       // log2(e) / sqrt(hd)
     float* out;
     uint32_t* counters;     // [B][ph]
-    float* partial;         // [CTA][2][kHeads][hd + 2]
+    float* partial;         // [CTA][2][heads of a pass][hd + 2]
     uint32_t* err;
 };
 
@@ -90,6 +89,11 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint4& a, uint32_t b
 }
 __device__ __forceinline__ void mma_u8u8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, const int4& c) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
+}
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, const int4& c) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
 }
@@ -164,26 +168,508 @@ struct Place {
     __device__ int mine(int j, int w) const { return j + ((w - j - pair) & (kWarps - 1)); }
 };
 
+// Zeroes the scales of a tile behind its `left` keys.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Args a) {
-    using X = Geo<HD>;
-    constexpr int NG = X::kNG, U = kKeys / 8;
+__device__ __forceinline__ void clear_scales(uint8_t* vs, int left, int lane) {
+    constexpr int NG = HD / FORGE_KV4_GROUP;
+#pragma unroll
+    for (int k = 0; k < kKeys * NG; k += 32)
+        if (k + lane >= left * NG) reinterpret_cast<uint16_t*>(vs)[k + lane] = 0;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
+    __syncwarp();
+}
+// The largest scales of a tile as bf16 bits: of its two groups, or of even and odd keys.
+template <int HD>
+__device__ __forceinline__ void largest_scales(const uint8_t* vs, int lane, uint32_t& s0, uint32_t& s1) {
+    constexpr int NG = HD / FORGE_KV4_GROUP;
+    uint32_t s = 0;
+#pragma unroll
+    for (int k = 0; k < kKeys * NG / 2; k += 32)
+        if (k + lane < kKeys * NG / 2) s = __vmaxu2(s, reinterpret_cast<const uint32_t*>(vs)[k + lane] & 0x7FFF7FFFu);
+    s0 = __reduce_max_sync(0xffffffffu, s & 0xffffu);
+    s1 = __reduce_max_sync(0xffffffffu, s >> 16);
+}
+// A key's scales, both groups' or one's.
+template <int NG>
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* base, int key) {
+    if constexpr (NG == 2) return reinterpret_cast<const uint32_t*>(base)[key];
+    else return reinterpret_cast<const uint16_t*>(base)[key];
+}
+
+// ---- up to 4 query heads: keys in the columns of B, digits in the rows of A
+// (rows r: digit 2, 1, 0 of head r % 4 for r < 4, r < 8, 8 <= r < 12)
+template <int HD>
+struct Many {
+    static constexpr int kHeads = kHeadsMany, kCtas = kCtasMany, NG = HD / FORGE_KV4_GROUP, U = kKeys / 8;
+    static constexpr int kSmem = 2 * NG * 512 + NG * 128 + 16;  // A operands of q [2 groups][32 lanes], sums to start from [groups][8], kMagic
+    const int warp, lane, g, t, h;
+    const float da, db, off;  // this lane's rows: digit a (2 or 1) and digit b (0, or none) of head h
+    const uint32_t sel;       // digits a of two words, then digits b
+    uint4* qs;
+    int4* from;
+    float fac, m;
+    F2 l, o[NG][8];  // o[group][2 k + b]: dims 64 i + 16 k + 4 t + b and + 2, this lane's digits' part
+
+    __device__ Many(uint8_t* smem, int warp, int lane)
+        : warp(warp), lane(lane), g(lane >> 2), t(lane & 3), h(g & 3), da(g < 4 ? 65536.f : 256.f), db(g < 4 ? 1.f : 0.f),
+          off(-12582912.f * (da + db)), sel(g < 4 ? 0x4062 : 0xBB51), qs(reinterpret_cast<uint4*>(smem)),
+          from(reinterpret_cast<int4*>(smem + 2 * NG * 512)) {
+        if (threadIdx.x == 0) from[8 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
+    }
+    __device__ int q_head() const { return h; }
+    __device__ bool holds() const { return g < 4; }      // the sums of head h, after sum_lanes()
+    __device__ bool first() const { return lane < 16 && t == 0; }  // of those that hold it
+
+    // q (dims 64 i + 16 t .. + 15 of head h) as A operands, dims 64 i + 16 t + 8 w + {0, 2, 4, 6} and {1, 3, 5, 7} (in
+    // shared memory, word w of group i from warp 2 i + w), and the sums that they start from
+    __device__ __forceinline__ void stage(const float4 (&v)[NG][4], float scale_log2) {
+        uint32_t mx = 0;  // largest |q| as bits
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mx = max(max(mx, __float_as_uint(fabsf(v[i][j].x))), __float_as_uint(fabsf(v[i][j].y)));
+                mx = max(max(mx, __float_as_uint(fabsf(v[i][j].z))), __float_as_uint(fabsf(v[i][j].w)));
+            }
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
+        const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
+        const float up = pow2i(23 - e);
+        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            int sa = 0, sb = 0;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const float4 lo4 = v[i][2 * w], hi4 = v[i][2 * w + 1];
+                const float x[8] = {lo4.x, lo4.z, hi4.x, hi4.z, lo4.y, lo4.w, hi4.y, hi4.w};  // even dims, odd dims
+                uint32_t da[8], db[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
+                    da[k] = g < 4 ? (n1 - d1) >> 8 : d1;
+                    db[k] = g < 4 ? d0 : 0;
+                }
+                const uint4 r = make_uint4(low_bytes(da), low_bytes(db), low_bytes(da + 4), low_bytes(db + 4));
+                if (warp == 2 * i + w) qs[(2 * i + w) * 32 + lane] = r;
+                sa = __dp4a((int)r.z, 0x01010101, __dp4a((int)r.x, 0x01010101, sa));
+                sb = __dp4a((int)r.w, 0x01010101, __dp4a((int)r.y, 0x01010101, sb));
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                sa += __shfl_xor_sync(0xffffffffu, sa, o);
+                sb += __shfl_xor_sync(0xffffffffu, sb, o);
+            }
+            if (warp == 0 && t == 0) from[8 * i + g] = make_int4(kMagic - 7 * sa, kMagic - 7 * sa, kMagic - 7 * sb, kMagic - 7 * sb);
+        }
+        m = -INFINITY;
+        l = F2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) o[i][n] = F2(0.f, 0.f);
+    }
+
+    __device__ __forceinline__ void tile(uint8_t* slot, int left) {
+        const uint8_t *kc = slot, *ks = slot + 2 * Geo<HD>::kCodes;
+        uint8_t* vs = slot + 2 * Geo<HD>::kCodes + Geo<HD>::kScales;
+        const uint8_t* krow = kc + (4 * (g >> 1) + (g & 1)) * (HD / 2) + 8 * t;  // this lane's keys of B, and of V's transposition
+        const uint8_t* vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
+        // ---- scores of keys 16 (u / 2) + 4 t + 2 (u % 2) + {0, 1}, head h, over fac
+        F2 x[U];
+#pragma unroll
+        for (int u0 = 0; u0 < U; u0 += 2) {
+            const Scales<NG> sk(ks, 2 * u0 + t);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const uint4 q0 = qs[2 * i * 32 + lane], q1 = qs[(2 * i + 1) * 32 + lane];
+                const int4 c0 = from[8 * i + g];
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(krow + (8 * u0 + 2 * f) * (HD / 2) + 32 * i);
+                    int c[4];
+                    mma_s8u8(c, q0, even(w.x), even(w.x >> 4), c0);
+                    mma_s8u8(c, q1, even(w.y), even(w.y >> 4), quad(c));
+                    // digit a times da + digit b times db; both offsets of 12582912 come off exactly with the first
+                    const F2 sum = fma2(float_bits(c[2], c[3]), F2(db, db), fma2(float_bits(c[0], c[1]), F2(da, da), F2(off, off)));
+                    x[u0 + f] = i ? fma2(sum, sk.of(f, i), x[u0 + f]) : sum * sk.of(f, i);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)  // the other digits
+            x[u] = x[u] + F2(__shfl_xor_sync(0xffffffffu, x[u].x(), 16), __shfl_xor_sync(0xffffffffu, x[u].y(), 16));
+        // ---- the tile's largest score and V scales; keys behind the last one count for nothing
+        if (left < kKeys) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                {
+                const int key = 8 * (u & ~1) + 2 * (u & 1) + 4 * t;
+                x[u] = F2(key < left ? x[u].x() : -INFINITY, key + 1 < left ? x[u].y() : -INFINITY);
+            }
+            clear_scales<HD>(vs, left, lane);
+        }
+        uint32_t smax0, smax1;
+        largest_scales<HD>(vs, lane, smax0, smax1);
+        float mx = fmaxf(x[0].x(), x[0].y());
+#pragma unroll
+        for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
+        // p = 2^(x - mx) <= 1
+        const float nmx = mx == -INFINITY ? 0.f : -mx;
+        F2 ls;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const F2 y = fma2(x[u], F2(fac, fac), F2(nmx, nmx));
+            x[u] = F2(ex2(y.x()), ex2(y.y()));
+            ls = u ? ls + x[u] : x[u];
+        }
+        // the tile's part of the sums, relative to the largest score so far
+        const float m_new = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : ex2(m - m_new);
+        const float beta = mx == -INFINITY ? 0.f : ex2(mx - m_new);
+        m = m_new;
+        l = fma2(l, F2(alpha, alpha), ls * F2(beta, beta));
+
+        // ---- O += P V, group by group
+        const Scales<NG> sv[U / 2] = {{vs, t}, {vs, 4 + t}, {vs, 8 + t}, {vs, 12 + t}};
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            // weights p sv unit < 2^23: 2^23 + weight has them in its low bits. (rcp is off by an ulp, the same for the tile)
+            const uint32_t sx = NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0;
+            const float smx = fmaxf(bf16_bits_to_f32((uint16_t)sx), 0x1p-100f), unit = rcp(smx) * (8388608.f * 255.f / 256.f);
+            const float wa = beta * smx * (256.f / 255.f / 8388608.f) * da, wb = beta * smx * (256.f / 255.f / 8388608.f) * db;
+            const int4 magic = from[8 * NG];
+            uint4 pa[U / 4];
+            int c7[4];
+#pragma unroll
+            for (int kb = 0; kb < U / 4; ++kb) {
+                uint32_t y[4];  // two digits of keys 32 kb + 16 (k / 2) + 4 t + 2 (k % 2) + {0, 1}
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const F2 n = fma2(x[4 * kb + k], sv[2 * kb + k / 2].of(k & 1, i) * F2(unit, unit), F2(8388608.f, 8388608.f));
+                    y[k] = prmt(__float_as_uint(n.x()), __float_as_uint(n.y()), sel);
+                }
+                pa[kb] = make_uint4(prmt(y[0], y[1], 0x5410), prmt(y[0], y[1], 0x7632), prmt(y[2], y[3], 0x5410), prmt(y[2], y[3], 0x7632));
+                mma_u8u8(c7, pa[kb], 0x07070707u, 0x07070707u, kb ? quad(c7) : magic);
+            }
+            // odd dims are 16 times; digit a's 7s and offset come off exactly, digit b's to below a unit of the weights
+            const float a7 = __int_as_float(c7[0]), b7 = __int_as_float(c7[2]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // 16 bytes of the group's 32
+                int c[4][4];
+#pragma unroll
+                for (int kb = 0; kb < U / 4; ++kb) {
+                    uint32_t r[4];
+                    load_transposed(r, vrow + 32 * kb * (HD / 2) + 32 * i + 16 * j);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        mma_u8u8(c[2 * k], pa[kb], even(r[k]), even(r[k + 2]), kb ? quad(c[2 * k]) : magic);
+                        mma_u8u8(c[2 * k + 1], pa[kb], odd16(r[k]), odd16(r[k + 2]), kb ? quad(c[2 * k + 1]) : magic);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float ua = n & 1 ? wa * 0.0625f : wa, ub = n & 1 ? wb * 0.0625f : wb;
+                    const float ma = n & 1 ? fmaf(a7, -16.f, 15.f * 12582912.f) : -a7, mb = n & 1 ? fmaf(b7, -16.f, 15.f * 12582912.f) : -b7;
+                    const F2 na = float_bits(c[n][0], c[n][1]) + F2(ma, ma);
+                    const F2 join = fma2(o[i][4 * j + n], F2(alpha, alpha), F2(mb * ub, mb * ub));
+                    o[i][4 * j + n] = fma2(na, F2(ua, ua), fma2(float_bits(c[n][2], c[n][3]), F2(ub, ub), join));
+                }
+            }
+            // (a scale that is no number has no digits)
+            if (sx >= 0x7F80u)
+#pragma unroll
+                for (int n = 0; n < 8; ++n) o[i][n] = F2(NAN, NAN);
+        }
+    }
+
+    __device__ __forceinline__ float sum_lanes() {  // returns the sum of the probabilities
+        float lw = l.x() + l.y();
+        lw += __shfl_xor_sync(0xffffffffu, lw, 1);
+        lw += __shfl_xor_sync(0xffffffffu, lw, 2);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                o[i][n] = o[i][n] + F2(__shfl_xor_sync(0xffffffffu, o[i][n].x(), 16), __shfl_xor_sync(0xffffffffu, o[i][n].y(), 16));
+        return lw;
+    }
+    __device__ __forceinline__ void put(float* row) const {
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; n += 2)
+                *reinterpret_cast<float4*>(row + 64 * i + 8 * n + 4 * t) = make_float4(o[i][n].x(), o[i][n + 1].x(), o[i][n].y(), o[i][n + 1].y());
+    }
+    __device__ __forceinline__ void add(float* row, float f, float fo) const {  // fo row + f o
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; n += 2) {
+                float4* at = reinterpret_cast<float4*>(row + 64 * i + 8 * n + 4 * t);
+                float4 v = *at;
+                v.x = fmaf(o[i][n].x(), f, v.x * fo); v.y = fmaf(o[i][n + 1].x(), f, v.y * fo);
+                v.z = fmaf(o[i][n].y(), f, v.z * fo); v.w = fmaf(o[i][n + 1].y(), f, v.w * fo);
+                *at = v;
+            }
+    }
+};
+
+// ---- one or two query heads: keys (of S) and dims (of O) in the rows of A,
+// digits in the columns of B (columns 4 h + 0, 1, 2: digits 2, 1, 0 of head h)
+template <int HD>
+struct Few {
+    static constexpr int kHeads = kHeadsFew, kCtas = kCtasFew, NG = HD / FORGE_KV4_GROUP, kBlocks = kKeys / 16;
+    static constexpr int kRowY = kKeys + 8;                              // words of a (head, group)'s weights, no bank twice
+    static constexpr int kY = kHeads * NG * kRowY * 4;                   // a warp's weights
+    static constexpr int kSmem = NG * 64 + 16 + kWarps * kY;             // sums to start from [groups][t], kMagic, weights
+    const int warp, lane, g, t, h, hq;
+    const float da, db, off;  // this lane's columns 2 t, 2 t + 1: digits 2 and 1 of head h, or digit 0 and nothing
+    const uint32_t sel;       // the digit of column g, of two words
+    int4* from;
+    uint32_t* ys;
+    uint2 qb[NG][2];
+    float fac, m;
+    F2 l, o[NG][4];  // o[group][2 k + b]: dims 64 i + 32 k + 2 g + b and + 16, this lane's digits' part
+
+    __device__ Few(uint8_t* smem, int warp, int lane)
+        : warp(warp), lane(lane), g(lane >> 2), t(lane & 3), h(t >> 1), hq(g >> 2), da(t & 1 ? 1.f : 65536.f),
+          db(t & 1 ? 0.f : 256.f), off(-12582912.f * (da + db)),
+          sel((g & 3) == 0 ? 0x62 : (g & 3) == 1 ? 0x51 : (g & 3) == 2 ? 0x40 : 0xFB), from(reinterpret_cast<int4*>(smem)),
+          ys(reinterpret_cast<uint32_t*>(smem + NG * 64 + 16 + warp * kY)) {
+        if (threadIdx.x == 0) from[4 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
+    }
+    __device__ int q_head() const { return hq; }
+    __device__ bool holds() const { return !(t & 1); }
+    __device__ bool first() const { return g == 0 && !(t & 1); }
+
+    // q (dims 64 i + 16 t .. + 15 of head g / 4) as B operands, dims 64 i + 16 t + 8 w + {0, 2, 4, 6} and {1, 3, 5, 7}, and
+    // the sums that the scores start from
+    __device__ __forceinline__ void stage(const float4 (&v)[NG][4], float scale_log2) {
+        uint32_t mx = 0;  // largest |q| as bits
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mx = max(max(mx, __float_as_uint(fabsf(v[i][j].x))), __float_as_uint(fabsf(v[i][j].y)));
+                mx = max(max(mx, __float_as_uint(fabsf(v[i][j].z))), __float_as_uint(fabsf(v[i][j].w)));
+            }
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
+        const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
+        const float up = pow2i(23 - e);
+        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
+        fac = __shfl_sync(0xffffffffu, fac, 16 * h);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const float4 lo4 = v[i][2 * w], hi4 = v[i][2 * w + 1];
+                const float x[8] = {lo4.x, lo4.z, hi4.x, hi4.z, lo4.y, lo4.w, hi4.y, hi4.w};  // even dims, odd dims
+                uint32_t d[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
+                    d[k] = (g & 3) == 0 ? (n1 - d1) >> 8 : (g & 3) == 1 ? d1 : (g & 3) == 2 ? d0 : 0;
+                }
+                qb[i][w] = make_uint2(low_bytes(d), low_bytes(d + 4));
+                sum = __dp4a((int)qb[i][w].x, 0x01010101, __dp4a((int)qb[i][w].y, 0x01010101, sum));
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int fa = kMagic - 7 * __shfl_sync(0xffffffffu, sum, 8 * t), fb = kMagic - 7 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            if (warp == 0 && g == 0) from[4 * i + t] = make_int4(fa, fb, fa, fb);
+        }
+        m = -INFINITY;
+        l = F2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) o[i][n] = F2(0.f, 0.f);
+    }
+
+    __device__ __forceinline__ void tile(uint8_t* slot, int left) {
+        const uint8_t *kc = slot, *ks = slot + 2 * Geo<HD>::kCodes;
+        uint8_t* vs = slot + 2 * Geo<HD>::kCodes + Geo<HD>::kScales;
+        const uint8_t *krow = kc + g * (HD / 2) + 8 * t, *vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
+        const int4 magic = from[4 * NG];
+        // ---- scores of keys 16 b + g and + 8, head h, over fac
+        F2 x[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const uint32_t s0 = scale_word<NG>(ks, 16 * b + g), s1 = scale_word<NG>(ks, 16 * b + 8 + g);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const uint2 w = *reinterpret_cast<const uint2*>(krow + 16 * b * (HD / 2) + 32 * i);
+                const uint2 z = *reinterpret_cast<const uint2*>(krow + (16 * b + 8) * (HD / 2) + 32 * i);
+                int c[4];
+                mma_u8s8(c, make_uint4(even(w.x), even(z.x), even(w.x >> 4), even(z.x >> 4)), qb[i][0].x, qb[i][0].y, from[4 * i + t]);
+                mma_u8s8(c, make_uint4(even(w.y), even(z.y), even(w.y >> 4), even(z.y >> 4)), qb[i][1].x, qb[i][1].y, quad(c));
+                // digits times da and db; both offsets of 12582912 come off exactly with the first
+                const F2 sum = fma2(float_bits(c[1], c[3]), F2(db, db), fma2(float_bits(c[0], c[2]), F2(da, da), F2(off, off)));
+                const F2 sp = i ? F2(bf16_hi_f32(s0), bf16_hi_f32(s1)) : F2(bf16_lo_f32(s0), bf16_lo_f32(s1));
+                x[b] = i ? fma2(sum, sp, x[b]) : sum * sp;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)  // the other digits
+            x[b] = x[b] + F2(__shfl_xor_sync(0xffffffffu, x[b].x(), 1), __shfl_xor_sync(0xffffffffu, x[b].y(), 1));
+        // ---- the tile's largest score and V scales; keys behind the last one count for nothing
+        if (left < kKeys) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+                x[b] = F2(16 * b + g < left ? x[b].x() : -INFINITY, 16 * b + 8 + g < left ? x[b].y() : -INFINITY);
+            clear_scales<HD>(vs, left, lane);
+        }
+        uint32_t smax0, smax1;
+        largest_scales<HD>(vs, lane, smax0, smax1);
+        float mx = fmaxf(x[0].x(), x[0].y());
+#pragma unroll
+        for (int b = 1; b < kBlocks; ++b) mx = max3(mx, x[b].x(), x[b].y());
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
+        // p = 2^(x - mx) <= 1
+        const float nmx = mx == -INFINITY ? 0.f : -mx;
+        F2 ls;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const F2 y = fma2(x[b], F2(fac, fac), F2(nmx, nmx));
+            x[b] = F2(ex2(y.x()), ex2(y.y()));
+            ls = b ? ls + x[b] : x[b];
+        }
+        // the tile's part of the sums, relative to the largest score so far
+        const float m_new = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : ex2(m - m_new);
+        const float beta = mx == -INFINITY ? 0.f : ex2(mx - m_new);
+        m = m_new;
+        l = fma2(l, F2(alpha, alpha), ls * F2(beta, beta));
+
+        // ---- weights p sv unit < 2^23, added to 2^23, of head h: lane t of the two for group t % 2 (both the same where there
+        // is one); through shared memory to the lanes whose column needs their keys
+        float smx[NG];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) smx[i] = fmaxf(bf16_bits_to_f32((uint16_t)(NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0)), 0x1p-100f);
+        {
+            const int i = NG == 2 ? t & 1 : 0;
+            const float unit = rcp(NG == 2 && i ? smx[NG - 1] : smx[0]) * (8388608.f * 255.f / 256.f);  // (off by an ulp, the same for the tile)
+            uint32_t* y = ys + (h * NG + i) * kRowY + g;
+            const uint16_t* sv = reinterpret_cast<const uint16_t*>(vs) + g * NG + i;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const F2 s2(bf16_bits_to_f32(sv[16 * b * NG]), bf16_bits_to_f32(sv[(16 * b + 8) * NG]));
+                const F2 n = fma2(x[b], s2 * F2(unit, unit), F2(8388608.f, 8388608.f));
+                y[16 * b] = __float_as_uint(n.x());
+                y[16 * b + 8] = __float_as_uint(n.y());
+            }
+        }
+        __syncwarp();
+
+        // ---- O += P V, group by group
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const float wa = beta * smx[i] * (256.f / 255.f / 8388608.f) * da, wb = beta * smx[i] * (256.f / 255.f / 8388608.f) * db;
+            uint2 pb[kKeys / 32];
+            int c7[4];
+#pragma unroll
+            for (int kb = 0; kb < kKeys / 32; ++kb) {
+                const uint32_t* y = ys + (hq * NG + i) * kRowY + 32 * kb + 4 * t;
+                const uint4 ya = *reinterpret_cast<const uint4*>(y), yb = *reinterpret_cast<const uint4*>(y + 16);
+                pb[kb].x = prmt(prmt(ya.x, ya.y, sel), prmt(ya.z, ya.w, sel), 0x5410);
+                pb[kb].y = prmt(prmt(yb.x, yb.y, sel), prmt(yb.z, yb.w, sel), 0x5410);
+                mma_u8u8(c7, make_uint4(0x07070707u, 0x07070707u, 0x07070707u, 0x07070707u), pb[kb].x, pb[kb].y, kb ? quad(c7) : magic);
+            }
+            const float a7 = __int_as_float(c7[0]), b7 = __int_as_float(c7[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // 16 bytes of the group's 32
+                int c[2][4];               // even dims; odd ones, times 16
+#pragma unroll
+                for (int kb = 0; kb < kKeys / 32; ++kb) {
+                    uint32_t r[4];
+                    load_transposed(r, vrow + 32 * kb * (HD / 2) + 32 * i + 16 * j);
+                    mma_u8u8(c[0], make_uint4(even(r[0]), even(r[1]), even(r[2]), even(r[3])), pb[kb].x, pb[kb].y, kb ? quad(c[0]) : magic);
+                    mma_u8u8(c[1], make_uint4(odd16(r[0]), odd16(r[1]), odd16(r[2]), odd16(r[3])), pb[kb].x, pb[kb].y, kb ? quad(c[1]) : magic);
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {  // the 7s and offsets come off exactly
+                    const float ua = n ? wa * 0.0625f : wa, ub = n ? wb * 0.0625f : wb;
+                    const float ma = n ? fmaf(a7, -16.f, 15.f * 12582912.f) : -a7, mb = n ? fmaf(b7, -16.f, 15.f * 12582912.f) : -b7;
+                    const F2 na = float_bits(c[n][0], c[n][2]) + F2(ma, ma), nb = float_bits(c[n][1], c[n][3]) + F2(mb, mb);
+                    F2& at = o[i][2 * j + n];
+                    at = fma2(na, F2(ua, ua), fma2(nb, F2(ub, ub), at * F2(alpha, alpha)));
+                }
+            }
+            // (a scale that is no number has no digits)
+            if ((NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0) >= 0x7F80u)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) o[i][n] = F2(NAN, NAN);
+        }
+    }
+
+    __device__ __forceinline__ float sum_lanes() {
+        float lw = l.x() + l.y();
+        lw += __shfl_xor_sync(0xffffffffu, lw, 4);
+        lw += __shfl_xor_sync(0xffffffffu, lw, 8);
+        lw += __shfl_xor_sync(0xffffffffu, lw, 16);
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                o[i][n] = o[i][n] + F2(__shfl_xor_sync(0xffffffffu, o[i][n].x(), 1), __shfl_xor_sync(0xffffffffu, o[i][n].y(), 1));
+        return lw;
+    }
+    __device__ __forceinline__ void put(float* row) const {
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float2* at = reinterpret_cast<float2*>(row + 64 * i + 32 * k + 2 * g);
+                at[0] = make_float2(o[i][2 * k].x(), o[i][2 * k + 1].x());
+                at[8] = make_float2(o[i][2 * k].y(), o[i][2 * k + 1].y());
+            }
+    }
+    __device__ __forceinline__ void add(float* row, float f, float fo) const {
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float2* at = reinterpret_cast<float2*>(row + 64 * i + 32 * k + 2 * g);
+                const float2 a = at[0], b = at[8];
+                at[0] = make_float2(fmaf(o[i][2 * k].x(), f, a.x * fo), fmaf(o[i][2 * k + 1].x(), f, a.y * fo));
+                at[8] = make_float2(fmaf(o[i][2 * k].y(), f, b.x * fo), fmaf(o[i][2 * k + 1].y(), f, b.y * fo));
+            }
+    }
+};
+
+template <int HD, typename Form>
+struct Layout : Geo<HD> {  // of shared memory
+    static constexpr int kRow = HD + 4;                                             // floats of a head in the join (no bank twice)
+    static constexpr int kOffForm = kWarps * kStages * Geo<HD>::kSlot;              // the form's
+    static constexpr int kOffRed = kOffForm + Form::kSmem;                          // [warp][heads][kRow] sums of warps
+    static constexpr int kOffMl = kOffRed + kJoin * Form::kHeads * kRow * 4;        // [warp][heads] m, then l
+    static constexpr int kOffBar = kOffMl + 2 * kJoin * Form::kHeads * 4;
+    static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
+};
+
+template <int HD, template <int> class Form>
+__global__ void __launch_bounds__(kThreads, Form<HD>::kCtas) k_kv4_decode(const Kv4Args a) {
+    using X = Layout<HD, Form<HD>>;
+    constexpr int NG = X::kNG, kHeads = Form<HD>::kHeads;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
     uint8_t* ring = smem + warp * kStages * X::kSlot;
-    uint4* qs = reinterpret_cast<uint4*>(smem + X::kOffQ);
-    int4* from = reinterpret_cast<int4*>(smem + X::kOffC);
     float* red = reinterpret_cast<float*>(smem + X::kOffRed);
     float* sm_m = reinterpret_cast<float*>(smem + X::kOffMl);
     float* sm_l = sm_m + kJoin * kHeads;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + X::kOffBar) + warp * kStages;
     __shared__ int s_last;
-    // this lane's rows of A: digit 2 or 1 of head h, and digit 0 or nothing
-    const int h = g & 3;
-    const float da = g < 4 ? 65536.f : 256.f, db = g < 4 ? 1.f : 0.f, off = -12582912.f * (da + db);
-    const uint32_t sel = g < 4 ? 0x4062 : 0xBB51;  // digits a of two words, then digits b
+    Form<HD> f(smem + X::kOffForm, warp, lane);
 
-    if (threadIdx.x == 0) from[8 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
@@ -300,12 +786,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         in_j += kWarps;
         ++n_in;
     };
-    // q of a pair (dims 64 i + 16 t .. + 15 of head h), loaded before what it can be loaded before
+    // q of a pair (dims 64 i + 16 t .. + 15 of the form's head), loaded before what it can be loaded before
     float4 v[NG][4];
     auto load_q = [&](const Place& p) {
         const int h0 = (p.pair % a.nhb) * kHeads;
-        const float* q = a.q + ((size_t)p.b * a.H + p.pair / a.nhb * a.G + h0 + h) * HD + 16 * t;
-        const bool mine = p.lo(start) < p.hi(end) && h < a.G - h0;
+        const float* q = a.q + ((size_t)p.b * a.H + p.pair / a.nhb * a.G + h0 + f.q_head()) * HD + 16 * t;
+        const bool mine = p.lo(start) < p.hi(end) && f.q_head() < a.G - h0;
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
@@ -324,60 +810,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
         const int kvh = at.pair / a.nhb, h0 = (at.pair % a.nhb) * kHeads, nh = min(kHeads, a.G - h0);
         const size_t qrow = (size_t)at.b * a.H + kvh * a.G + h0;
 
-        // q as A operands, dims 64 i + 16 t + 8 w + {0, 2, 4, 6} and {1, 3, 5, 7} (in shared memory, word w of group i from
-        // warp 2 i + w), and the sums that they start from
-        float fac;
-        {
-            uint32_t mx = 0;  // largest |q| as bits
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mx = max(max(mx, __float_as_uint(fabsf(v[i][j].x))), __float_as_uint(fabsf(v[i][j].y)));
-                    mx = max(max(mx, __float_as_uint(fabsf(v[i][j].z))), __float_as_uint(fabsf(v[i][j].w)));
-                }
-            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
-            const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
-            const float up = pow2i(23 - e);
-            fac = mx >= 0x7F800000u ? NAN : a.scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                int sa = 0, sb = 0;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const float4 lo4 = v[i][2 * w], hi4 = v[i][2 * w + 1];
-                    const float x[8] = {lo4.x, lo4.z, hi4.x, hi4.z, lo4.y, lo4.w, hi4.y, hi4.w};  // even dims, odd dims
-                    uint32_t da[8], db[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
-                        da[k] = g < 4 ? (n1 - d1) >> 8 : d1;
-                        db[k] = g < 4 ? d0 : 0;
-                    }
-                    const uint4 r = make_uint4(low_bytes(da), low_bytes(db), low_bytes(da + 4), low_bytes(db + 4));
-                    if (warp == 2 * i + w) qs[(2 * i + w) * 32 + lane] = r;
-                    sa = __dp4a((int)r.z, 0x01010101, __dp4a((int)r.x, 0x01010101, sa));
-                    sb = __dp4a((int)r.w, 0x01010101, __dp4a((int)r.y, 0x01010101, sb));
-                }
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    sa += __shfl_xor_sync(0xffffffffu, sa, o);
-                    sb += __shfl_xor_sync(0xffffffffu, sb, o);
-                }
-                if (warp == 0 && t == 0) from[8 * i + g] = make_int4(kMagic - 7 * sa, kMagic - 7 * sa, kMagic - 7 * sb, kMagic - 7 * sb);
-            }
-        }
+        f.stage(v, a.scale_log2);
         __syncthreads();
-
-        float m = -INFINITY;
-        F2 l(0.f, 0.f), o[NG][8];  // o[group][2 k + b]: dims 64 i + 16 k + 4 t + b and + 2, this lane's digits' part
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int n = 0; n < 8; ++n) o[i][n] = F2(0.f, 0.f);
-
 #pragma unroll 1
         for (int j = at.mine(j0, warp); j < j1; j += kWarps) {
             if (dead) break;
@@ -387,178 +821,41 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
                 while (++n_out < n_in) mbar_wait(&full[n_out % kStages], (n_out / kStages) & 1, a.err);
                 break;
             }
-            const uint8_t* kc = ring + s * X::kSlot;
-            const uint8_t* ks = kc + 2 * X::kCodes;
-            const uint8_t* krow = kc + (4 * (g >> 1) + (g & 1)) * (HD / 2) + 8 * t;  // this lane's keys of B, and of V's transposition
-            const uint8_t* vrow = kc + X::kCodes + lane * (HD / 2);
-            uint8_t* vs = const_cast<uint8_t*>(ks) + X::kScales;
             const int left = j + 1 < at.n ? kKeys : a.pos[at.b] + 1 - j * kKeys;  // keys of the tile
 
-            // ---- scores of keys 16 (u / 2) + 4 t + 2 (u % 2) + {0, 1}, head h, over fac
-            F2 x[U];
-#pragma unroll
-            for (int u0 = 0; u0 < U; u0 += 2) {
-                const Scales<NG> sk(ks, 2 * u0 + t);
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const uint4 q0 = qs[2 * i * 32 + lane], q1 = qs[(2 * i + 1) * 32 + lane];
-                    const int4 c0 = from[8 * i + g];
-#pragma unroll
-                    for (int f = 0; f < 2; ++f) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(krow + (8 * u0 + 2 * f) * (HD / 2) + 32 * i);
-                        int c[4];
-                        mma_s8u8(c, q0, even(w.x), even(w.x >> 4), c0);
-                        mma_s8u8(c, q1, even(w.y), even(w.y >> 4), quad(c));
-                        // digit a times da + digit b times db; both offsets of 12582912 come off exactly with the first
-                        const F2 sum = fma2(float_bits(c[2], c[3]), F2(db, db), fma2(float_bits(c[0], c[1]), F2(da, da), F2(off, off)));
-                        x[u0 + f] = i ? fma2(sum, sk.of(f, i), x[u0 + f]) : sum * sk.of(f, i);
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)  // the other digits
-                x[u] = x[u] + F2(__shfl_xor_sync(0xffffffffu, x[u].x(), 16), __shfl_xor_sync(0xffffffffu, x[u].y(), 16));
-            // ---- the tile's largest score and V scales; keys behind the last one count for nothing
-            if (left < kKeys) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    {
-                    const int key = 8 * (u & ~1) + 2 * (u & 1) + 4 * t;
-                    x[u] = F2(key < left ? x[u].x() : -INFINITY, key + 1 < left ? x[u].y() : -INFINITY);
-                }
-#pragma unroll
-                for (int k = 0; k < kKeys * NG; k += 32)
-                    if (k + lane >= left * NG) reinterpret_cast<uint16_t*>(vs)[k + lane] = 0;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
-                __syncwarp();
-            }
-            uint32_t smax = 0;  // bf16 bits: of group 0 and 1, or of even and odd keys
-#pragma unroll
-            for (int k = 0; k < kKeys * NG / 2; k += 32)
-                if (k + lane < kKeys * NG / 2) smax = __vmaxu2(smax, reinterpret_cast<const uint32_t*>(vs)[k + lane] & 0x7FFF7FFFu);
-            const uint32_t smax0 = __reduce_max_sync(0xffffffffu, smax & 0xffffu), smax1 = __reduce_max_sync(0xffffffffu, smax >> 16);
-            float mx = fmaxf(x[0].x(), x[0].y());
-#pragma unroll
-            for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
-            // p = 2^(x - mx) <= 1
-            const float nmx = mx == -INFINITY ? 0.f : -mx;
-            F2 ls;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const F2 y = fma2(x[u], F2(fac, fac), F2(nmx, nmx));
-                x[u] = F2(ex2(y.x()), ex2(y.y()));
-                ls = u ? ls + x[u] : x[u];
-            }
-            // the tile's part of the sums, relative to the largest score so far
-            const float m_new = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : ex2(m - m_new);
-            const float beta = mx == -INFINITY ? 0.f : ex2(mx - m_new);
-            m = m_new;
-            l = fma2(l, F2(alpha, alpha), ls * F2(beta, beta));
-
-            // ---- O += P V, group by group
-            const Scales<NG> sv[U / 2] = {{vs, t}, {vs, 4 + t}, {vs, 8 + t}, {vs, 12 + t}};
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                // weights p sv unit < 2^23: 2^23 + weight has them in its low bits. (rcp is off by an ulp, the same for the tile)
-                const uint32_t sx = NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0;
-                const float smx = fmaxf(bf16_bits_to_f32((uint16_t)sx), 0x1p-100f), unit = rcp(smx) * (8388608.f * 255.f / 256.f);
-                const float wa = beta * smx * (256.f / 255.f / 8388608.f) * da, wb = beta * smx * (256.f / 255.f / 8388608.f) * db;
-                const int4 magic = from[8 * NG];
-                uint4 pa[U / 4];
-                int c7[4];
-#pragma unroll
-                for (int kb = 0; kb < U / 4; ++kb) {
-                    uint32_t y[4];  // two digits of keys 32 kb + 16 (k / 2) + 4 t + 2 (k % 2) + {0, 1}
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const F2 n = fma2(x[4 * kb + k], sv[2 * kb + k / 2].of(k & 1, i) * F2(unit, unit), F2(8388608.f, 8388608.f));
-                        y[k] = prmt(__float_as_uint(n.x()), __float_as_uint(n.y()), sel);
-                    }
-                    pa[kb] = make_uint4(prmt(y[0], y[1], 0x5410), prmt(y[0], y[1], 0x7632), prmt(y[2], y[3], 0x5410), prmt(y[2], y[3], 0x7632));
-                    mma_u8u8(c7, pa[kb], 0x07070707u, 0x07070707u, kb ? quad(c7) : magic);
-                }
-                // odd dims are 16 times; digit a's 7s and offset come off exactly, digit b's to below a unit of the weights
-                const float a7 = __int_as_float(c7[0]), b7 = __int_as_float(c7[2]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {  // 16 bytes of the group's 32
-                    int c[4][4];
-#pragma unroll
-                    for (int kb = 0; kb < U / 4; ++kb) {
-                        uint32_t r[4];
-                        load_transposed(r, vrow + 32 * kb * (HD / 2) + 32 * i + 16 * j);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            mma_u8u8(c[2 * k], pa[kb], even(r[k]), even(r[k + 2]), kb ? quad(c[2 * k]) : magic);
-                            mma_u8u8(c[2 * k + 1], pa[kb], odd16(r[k]), odd16(r[k + 2]), kb ? quad(c[2 * k + 1]) : magic);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float ua = n & 1 ? wa * 0.0625f : wa, ub = n & 1 ? wb * 0.0625f : wb;
-                        const float ma = n & 1 ? fmaf(a7, -16.f, 15.f * 12582912.f) : -a7, mb = n & 1 ? fmaf(b7, -16.f, 15.f * 12582912.f) : -b7;
-                        const F2 na = float_bits(c[n][0], c[n][1]) + F2(ma, ma);
-                        const F2 join = fma2(o[i][4 * j + n], F2(alpha, alpha), F2(mb * ub, mb * ub));
-                        o[i][4 * j + n] = fma2(na, F2(ua, ua), fma2(float_bits(c[n][2], c[n][3]), F2(ub, ub), join));
-                    }
-                }
-                // (a scale that is no number has no digits)
-                if (sx >= 0x7F80u)
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) o[i][n] = F2(NAN, NAN);
-            }
-            if (poison >> s & 1) l = F2(NAN, NAN);
+            f.tile(ring + s * X::kSlot, left);
+            if (poison >> s & 1) f.l = F2(NAN, NAN);
             ++n_out;
             __syncwarp();
             issue();
         }
-        if (dead) l = F2(NAN, NAN);
+        if (dead) f.l = F2(NAN, NAN);
         following.next(a);
         load_q(following);
 
         // ---- join the warps: the upper half's sums into the lower half's, then those over the CTA
-        float lw = l.x() + l.y();
-        lw += __shfl_xor_sync(0xffffffffu, lw, 1);
-        lw += __shfl_xor_sync(0xffffffffu, lw, 2);
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-                o[i][n] = o[i][n] + F2(__shfl_xor_sync(0xffffffffu, o[i][n].x(), 16), __shfl_xor_sync(0xffffffffu, o[i][n].y(), 16));
-        const int slot = warp % kJoin * kHeads + h;
-        float* mine = red + slot * X::kRow + 4 * t;
-        if (warp >= kJoin && g < nh) {
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-#pragma unroll
-                for (int n = 0; n < 8; n += 2)
-                    *reinterpret_cast<float4*>(mine + 64 * i + 8 * n) = make_float4(o[i][n].x(), o[i][n + 1].x(), o[i][n].y(), o[i][n + 1].y());
-            if (t == 0) {
-                sm_m[slot] = m;
+        const float lw = f.sum_lanes();
+        const int slot = warp % kJoin * kHeads + f.h;
+        float* mine = red + slot * X::kRow;
+        const bool holds = f.holds() && f.h < nh;
+        if (warp >= kJoin && holds) {
+            f.put(mine);
+            if (f.first()) {
+                sm_m[slot] = f.m;
                 sm_l[slot] = lw;
             }
         }
         __syncthreads();
         const float mo = sm_m[slot], lo = sm_l[slot];
         __syncwarp();
-        if (warp < kJoin && g < nh) {
-            const float mj = fmaxf(m, mo);
-            const float f = m == -INFINITY ? 0.f : ex2(m - mj), fo = mo == -INFINITY ? 0.f : ex2(mo - mj);
-            if (t == 0) {
+        if (warp < kJoin && holds) {
+            const float mj = fmaxf(f.m, mo);
+            const float fm = f.m == -INFINITY ? 0.f : ex2(f.m - mj), fo = mo == -INFINITY ? 0.f : ex2(mo - mj);
+            if (f.first()) {
                 sm_m[slot] = mj;
-                sm_l[slot] = isnan(lo) || isnan(lw) ? NAN : fmaf(lw, f, lo * fo);
+                sm_l[slot] = isnan(lo) || isnan(lw) ? NAN : fmaf(lw, fm, lo * fo);
             }
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-#pragma unroll
-                for (int n = 0; n < 8; n += 2) {
-                    float4 v = *reinterpret_cast<const float4*>(mine + 64 * i + 8 * n);
-                    v.x = fmaf(o[i][n].x(), f, v.x * fo); v.y = fmaf(o[i][n + 1].x(), f, v.y * fo);
-                    v.z = fmaf(o[i][n].y(), f, v.z * fo); v.w = fmaf(o[i][n + 1].y(), f, v.w * fo);
-                    *reinterpret_cast<float4*>(mine + 64 * i + 8 * n) = v;
-                }
+            f.add(mine, fm, fo);
         }
         __syncthreads();
         const int unit0 = at.base + kPairUnits, cfirst = unit0 / per, clast = (unit0 + at.n - 1) / per;
@@ -572,10 +869,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_kv4_decode(const Kv4Ar
 #pragma unroll
             for (int w = 0; w < kJoin; ++w) {
                 const float mw = sm_m[w * kHeads + h], lv = sm_l[w * kHeads + h];
-                const float f = mw == -INFINITY ? 0.f : ex2(mw - mj);
-                lj = isnan(lv) ? lv : fmaf(lv, f, lj);
+                const float fw = mw == -INFINITY ? 0.f : ex2(mw - mj);
+                lj = isnan(lv) ? lv : fmaf(lv, fw, lj);
                 const float4 r = *reinterpret_cast<const float4*>(red + (w * kHeads + h) * X::kRow + d);
-                v.x = fmaf(r.x, f, v.x); v.y = fmaf(r.y, f, v.y); v.z = fmaf(r.z, f, v.z); v.w = fmaf(r.w, f, v.w);
+                v.x = fmaf(r.x, fw, v.x); v.y = fmaf(r.y, fw, v.y); v.z = fmaf(r.z, fw, v.z); v.w = fmaf(r.w, fw, v.w);
             }
             const float il = 1.f / lj;
             v.x *= il; v.y *= il; v.z *= il; v.w *= il;
@@ -656,25 +953,35 @@ int configure() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return forge_fail(-1, "forge_flash_decode_kv4: no device");
     if (done[dev]) return 0;
-    cudaError_t e = cudaFuncSetAttribute(k_kv4_decode<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<64>::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv4_decode<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<128>::kSmem);
-    for (auto k : {k_kv4_decode<64>, k_kv4_decode<128>})
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto kernel, int smem) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    };
+    set(k_kv4_decode<64, Few>, Layout<64, Few<64>>::kSmem);
+    set(k_kv4_decode<128, Few>, Layout<128, Few<128>>::kSmem);
+    set(k_kv4_decode<64, Many>, Layout<64, Many<64>>::kSmem);
+    set(k_kv4_decode<128, Many>, Layout<128, Many<128>>::kSmem);
     if (e != cudaSuccess) return forge_fail(-1, "forge_flash_decode_kv4: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
     return 0;
 }
 
+// Passes over a KV head's keys for the G query heads that read it.
+int heads_of_a_pass(int G) { return G <= kHeadsFew ? kHeadsFew : kHeadsMany; }
+int passes(int G) { return (G + heads_of_a_pass(G) - 1) / heads_of_a_pass(G); }
+
 int64_t counter_bytes(int B, int H, int Hkv) {
-    const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + kHeads - 1) / kHeads);
+    const int64_t pairs = (int64_t)B * Hkv * passes(H / Hkv);
     return (pairs * 4 + 255) / 256 * 256;
 }
-constexpr int kMaxCtas = 148 * kCtasPerSm;  // a B200's; fixed so that workspace sizes do not depend on the device
+// A B200's CTAs; fixed so that workspace sizes do not depend on the device.
+int most_ctas(int G) { return 148 * (heads_of_a_pass(G) == kHeadsFew ? kCtasFew : kCtasMany); }
 }  // namespace
 
 extern "C" FORGE_API int64_t forge_flash_decode_kv4_workspace_bytes(int B, int H, int n_kv_head, int head_dim) {
     if (B <= 0 || H <= 0 || n_kv_head <= 0 || H % n_kv_head || (head_dim != 64 && head_dim != 128)) return -1;
-    return counter_bytes(B, H, n_kv_head) + (int64_t)kMaxCtas * 2 * kHeads * (head_dim + 2) * 4;
+    return counter_bytes(B, H, n_kv_head) + (int64_t)most_ctas(H / n_kv_head) * 2 * heads_of_a_pass(H / n_kv_head) * (head_dim + 2) * 4;
 }
 
 extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* cache, const int32_t* seq,
@@ -685,7 +992,7 @@ extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* 
         (!seq && B > cache->n_seq) || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15))
         return forge_fail(FORGE_INVALID_ARGS, "forge_flash_decode_kv4: bad args (arrays 16-byte aligned, H a multiple of the KV heads)");
     const int hd = cache->head_dim, cap = cache->table ? cache->max_pages * cache->page_tokens : cache->lmax;
-    const int64_t units = (int64_t)B * cache->n_kv_head * ((H / cache->n_kv_head + kHeads - 1) / kHeads) * ((cap + kKeys - 1) / kKeys + kPairUnits);
+    const int64_t units = (int64_t)B * cache->n_kv_head * passes(H / cache->n_kv_head) * ((cap + kKeys - 1) / kKeys + kPairUnits);
     if (units > (1ll << 30))
         return forge_fail(FORGE_INVALID_ARGS, "forge_flash_decode_kv4: B x KV heads x rows of a sequence is too large (%lld tiles of 64 keys)", (long long)units);
     uint32_t* err = forge_ops_err_word();
@@ -694,7 +1001,7 @@ extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* 
     Kv4Args a{};
     a.c = *cache; a.q = q; a.seq = seq; a.pos = pos; a.B = B; a.H = H;
     a.G = H / cache->n_kv_head;
-    a.nhb = (a.G + kHeads - 1) / kHeads;
+    a.nhb = passes(a.G);
     a.ph = cache->n_kv_head * a.nhb;
     a.cap = cap;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
@@ -703,8 +1010,14 @@ extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* 
     a.partial = (float*)((char*)workspace + counter_bytes(B, H, cache->n_kv_head));
     // no more CTAs than the longest sequences could feed
     const int64_t most = (units + kMinUnits - 1) / kMinUnits;
-    const int grid = (int)(most < kMaxCtas ? most : kMaxCtas);
-    if (hd == 128) k_kv4_decode<128><<<grid, kThreads, Geo<128>::kSmem, (cudaStream_t)stream>>>(a);
-    else k_kv4_decode<64><<<grid, kThreads, Geo<64>::kSmem, (cudaStream_t)stream>>>(a);
+    const int grid = (int)std::min<int64_t>(most, most_ctas(a.G));
+    auto go = [&](auto kernel, int smem) { kernel<<<grid, kThreads, smem, (cudaStream_t)stream>>>(a); };
+    if (heads_of_a_pass(a.G) == kHeadsFew) {
+        if (hd == 128) go(k_kv4_decode<128, Few>, Layout<128, Few<128>>::kSmem);
+        else go(k_kv4_decode<64, Few>, Layout<64, Few<64>>::kSmem);
+    } else {
+        if (hd == 128) go(k_kv4_decode<128, Many>, Layout<128, Many<128>>::kSmem);
+        else go(k_kv4_decode<64, Many>, Layout<64, Many<64>>::kSmem);
+    }
     return forge_check_launch("forge_flash_decode_kv4");
 }

@@ -21,16 +21,16 @@
 //
 // Two forms, for how many query heads read a KV head. Up to 2: keys and dims
 // are the 16 rows of A and the digits of both heads 6 of the 8 columns, so a lane
-// has half of a tile's scores, exponentials and sums of the other form, about
-// 560 instructions for 64 keys of 128 dims, and 165 registers let 3 CTAs share
-// an SM. 3 and more: 4 heads' digits are 12 of the 16 rows, keys and dims the 8
-// columns, about 840 instructions, fewer than two passes of the first form, and
-// the keys are read once for the 4. Measured, 64 sequences of 4096 with 40 heads
+// has half of a tile's scores, exponentials and sums of the other form: 760
+// instructions for 64 keys of 128 dims (pairs' starts and joins among them), and
+// 165 registers let 3 CTAs share an SM. 3 and more: 4 heads' digits are 12 of
+// the 16 rows, keys and dims the 8 columns: 845 instructions, fewer than two
+// passes of the first form, and the keys are read once for the 4. Measured, 64 sequences of 4096 with 40 heads
 // of 128, each reading its own KV head (1.43 GB; 218 us at the rate of a copy):
-// 220 us in the first form, 6.5 TB/s, bound by HBM; 265 in the second, bound by
-// issue and latencies (0.49 of the issue slots with 2 warps a scheduler; 3 would
-// have 168 registers and spill) and shared-memory banks (0.61 of the wavefronts:
-// ldmatrix's rows 64 bytes apart share them). The same products in fp16, q and
+// 220 us in the first form, 6.5 TB/s, bound by HBM, next by shared-memory banks
+// (0.74 of the wavefronts: ldmatrix's rows 64 bytes apart share them); 265 in the
+// second, bound by issue and latencies (0.49 of the issue slots with 2 warps a
+// scheduler; 3 would have 168 registers and spill). The same products in fp16, q and
 // weights as pairs of fp16, took 379. Short contexts are a chain of latencies:
 // 10 us for one sequence of 2048.
 //

@@ -70,6 +70,46 @@ def test_decode_with_large_query_channels(forge, cuda):
     kv4.check(kv4.decode(forge, cuda, cache, q, pos), (out, tol))
 
 
+@pytest.mark.parametrize("hd,H,Hkv", [(64, 4, 4), (64, 6, 3), (128, 8, 4), (128, 2, 1), (64, 1, 1), (64, 9, 3)])
+@pytest.mark.parametrize("page", [0, 8, 24])
+def test_decode_few_heads(forge, cuda, hd, H, Hkv, page):
+    """One, two and three query heads a KV head, at lengths around every boundary and long ones that CTAs share."""
+    pos = [0, -1, 1, 6, 7, 8, 15, 16, 31, 32, 47, 62, 63, 64, 65, 127, 128, 500, 1151, 1100]
+    cache = kv4.Cache(forge, cuda, len(pos), Hkv, hd, 1152, page, seed=hd + H)
+    q = np.random.default_rng(H).standard_normal((len(pos), H, hd)).astype(np.float32) * 2
+    got = kv4.decode(forge, cuda, cache, q, pos)
+    forge.check(forge.lib().forge_ops_check(), "error word")
+    kv4.check(got, kv4.reference(cache, q, pos))
+    assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("hd,H,Hkv", [(128, 2, 2), (64, 4, 2)])
+def test_decode_few_heads_masked_rows(forge, cuda, hd, H, Hkv):
+    """NaN scales behind the last position are not seen; a NaN or an infinity in q is its own head's; a NaN scale of V its
+    group's."""
+    import torch
+    G = H // Hkv
+    cache = kv4.Cache(forge, cuda, 2, Hkv, hd, 256, 0, seed=12)
+    pos = [77, 200]
+    q = np.random.default_rng(7).standard_normal((2, H, hd)).astype(np.float32)
+    want = kv4.reference(cache, q, pos)
+    for kv in range(2):
+        s = cache.scales[kv].copy()
+        for b, p in enumerate(pos):
+            s[b, :, p + 1:] = np.nan
+        cache.d[2 + kv].copy_(torch.from_numpy(kv4.bits16(s).view(np.int16)))
+    kv4.check(kv4.decode(forge, cuda, cache, q, pos), want)
+    bad = q.copy()
+    bad[0, 0, 3], bad[1, H - 1, 9] = np.nan, np.inf
+    got = kv4.decode(forge, cuda, cache, bad, pos)
+    nan = np.isnan(got)
+    assert nan[0, 0].all() and nan[1, H - 1].all() and not nan[0, 1:].any() and not nan[1, :H - 1].any()
+    cache.d[3].view(*cache.scales[1].shape)[1, 0, 40, -1] = 0x7FC0
+    got = kv4.decode(forge, cuda, cache, q, pos)
+    assert np.isnan(got[1, :G, -64:]).all() and np.isfinite(got[1, :G, :-64]).all()
+    assert np.isfinite(got[0]).all() and np.isfinite(got[1, G:]).all()
+
+
 def test_decode_forty_heads_of_one_kv_head(forge, cuda):
     cache = kv4.Cache(forge, cuda, 2, 1, 64, 3000, 8, seed=6)
     q = np.random.default_rng(6).standard_normal((2, 41, 64)).astype(np.float32)

@@ -971,17 +971,16 @@ int configure() {
 int heads_of_a_pass(int G) { return G <= kHeadsFew ? kHeadsFew : kHeadsMany; }
 int passes(int G) { return (G + heads_of_a_pass(G) - 1) / heads_of_a_pass(G); }
 
-int64_t counter_bytes(int B, int H, int Hkv) {
-    const int64_t pairs = (int64_t)B * Hkv * passes(H / Hkv);
-    return (pairs * 4 + 255) / 256 * 256;
-}
 // A B200's CTAs; fixed so that workspace sizes do not depend on the device.
 int most_ctas(int G) { return 148 * (heads_of_a_pass(G) == kHeadsFew ? kCtasFew : kCtasMany); }
+// The partials, at the workspace's start; the counters behind them lie in the same place for every batch, so that one
+// call's partials never become another's counters.
+int64_t partial_bytes(int G, int hd) { return (int64_t)most_ctas(G) * 2 * heads_of_a_pass(G) * (hd + 2) * 4; }
 }  // namespace
-
 extern "C" FORGE_API int64_t forge_flash_decode_kv4_workspace_bytes(int B, int H, int n_kv_head, int head_dim) {
     if (B <= 0 || H <= 0 || n_kv_head <= 0 || H % n_kv_head || (head_dim != 64 && head_dim != 128)) return -1;
-    return counter_bytes(B, H, n_kv_head) + (int64_t)most_ctas(H / n_kv_head) * 2 * heads_of_a_pass(H / n_kv_head) * (head_dim + 2) * 4;
+    const int64_t pairs = (int64_t)B * n_kv_head * passes(H / n_kv_head);
+    return partial_bytes(H / n_kv_head, head_dim) + (pairs * 4 + 255) / 256 * 256;
 }
 
 extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* cache, const int32_t* seq,
@@ -1006,8 +1005,8 @@ extern "C" FORGE_API int forge_flash_decode_kv4(const float* q, const ForgeKv4* 
     a.cap = cap;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)hd));
     a.out = out; a.err = err;
-    a.counters = (uint32_t*)workspace;
-    a.partial = (float*)((char*)workspace + counter_bytes(B, H, cache->n_kv_head));
+    a.partial = (float*)workspace;
+    a.counters = (uint32_t*)((char*)workspace + partial_bytes(a.G, hd));
     // no more CTAs than the longest sequences could feed
     const int64_t most = (units + kMinUnits - 1) / kMinUnits;
     const int grid = (int)std::min<int64_t>(most, most_ctas(a.G));

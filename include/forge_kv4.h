@@ -71,8 +71,10 @@ int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos
  * sequence's output NaN.
  * workspace: forge_flash_decode_kv4_workspace_bytes(...) bytes, 16-byte
  * aligned, zeroed once before first use (every call leaves its counters at
- * zero); calls that may overlap on the GPU, captured graphs among them, need
- * a workspace each. */
+ * zero, unless a wait ran out, which forge_ops_check() reports: zero it again
+ * then); one for the largest batch serves smaller ones of the same heads and
+ * head_dim. Calls that may overlap on the GPU, captured graphs among them,
+ * need a workspace each. */
 int64_t forge_flash_decode_kv4_workspace_bytes(int B, int H, int n_kv_head, int head_dim);
 int forge_flash_decode_kv4(const float* q, const ForgeKv4* cache, const int32_t* seq, const int32_t* pos, int B, int H,
                            float* out, void* workspace, void* stream);

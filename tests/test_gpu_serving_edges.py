@@ -116,6 +116,20 @@ def test_decode_forty_heads_of_one_kv_head(forge, cuda):
     kv4.check(kv4.decode(forge, cuda, cache, q, [2900, 64]), kv4.reference(cache, q, [2900, 64]))
 
 
+@pytest.mark.parametrize("H,Hkv", [(64, 16), (32, 32)])
+def test_decode_workspace_of_the_largest_batch(forge, cuda, H, Hkv):
+    """One workspace, sized for the largest batch, for batches of several sizes in turn."""
+    import torch
+    hd, most = 64, 40
+    cache = kv4.Cache(forge, cuda, 4, Hkv, hd, 640, 0, seed=13)
+    q = np.random.default_rng(13).standard_normal((most, H, hd)).astype(np.float32)
+    pos, seq = [639 - 7 * b for b in range(most)], [b % 4 for b in range(most)]
+    out, tol = kv4.reference(cache, q, pos, seq)
+    ws = torch.zeros(forge.lib().forge_flash_decode_kv4_workspace_bytes(most, H, Hkv, hd), dtype=torch.uint8, device=cuda)
+    for B in (1, 3, 40, 2, 17, 40):
+        kv4.check(kv4.decode(forge, cuda, cache, q[:B], pos[:B], seq[:B], ws), (out[:B], tol[:B]))
+
+
 def test_decode_on_two_streams_at_once(forge, cuda):
     """Two calls in flight, each with its own workspace, repeated."""
     import torch

@@ -674,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, Form<HD>::kCtas) k_kv4_decode(const 
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
     }
+    __syncwarp();  // (before the lane that issues the first copies arrives on them)
 
     // ---- the line's length; sequences without tiles are answered here
     const int n0 = lane < a.B ? tiles_of(a, lane) : 0;

@@ -46,6 +46,7 @@
 #include "common.cuh"
 #include "f32x2.cuh"
 #include "forge_internal.h"
+#include "ring.cuh"
 #include "../../include/forge_b200.h"
 #include "../../include/forge_kv4.h"
 
@@ -818,8 +819,8 @@ __global__ void __launch_bounds__(kThreads, Form<HD>::kCtas) k_kv4_decode(const 
             if (dead) break;
             const int s = n_out % kStages;
             if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (n_out / kStages) & 1, a.err))) {
-                dead = true;  // the copies in flight land before the CTA exits
-                while (++n_out < n_in) mbar_wait(&full[n_out % kStages], (n_out / kStages) & 1, a.err);
+                dead = true;  // the copies in flight get the same time again to land before the CTA exits
+                ring_drain<kStages>(n_out, n_in, [&](int slot, int parity) { mbar_wait(&full[slot], parity, a.err); });
                 break;
             }
             const int left = j + 1 < at.n ? kKeys : a.pos[at.b] + 1 - j * kKeys;  // keys of the tile

@@ -9,10 +9,13 @@
 //   S: q times a power of two as 24-bit integers, signed digits; -7 sum q is
 //      in the initial sum. A group's sum is multiplied by the key's scale in
 //      fp32.
-//   O: the weights p_j sv_jg of a tile as integers below 2^23, p relative to
-//      the tile's own maximum and sv to its largest scale: added to 2^23 their
-//      digits are the fp32's low bytes. ldmatrix transposes V's bytes, so that a
-//      register holds a byte of four keys; odd dims stay times 16 in theirs.
+//   O: the weights p_j sv_jg of a tile as integers below 2^23, relative to the
+//      largest of them (of a head and group): added to 2^23 their digits are the
+//      fp32's low bytes. A unit of p's and sv's own maxima would lose the bits
+//      of a sink, a key that has the weight but not the scale. Groups of zeros,
+//      whose scale is 1 by the format, are left out of it. ldmatrix transposes
+//      V's bytes, so that a register holds a byte of four keys; odd dims stay
+//      times 16 in theirs.
 //      One more product, with a constant 7, gives 7 times the sum of the
 //      weights, taken off exactly before the tile joins O in fp32.
 //
@@ -179,17 +182,36 @@ __device__ __forceinline__ void clear_scales(uint8_t* vs, int left, int lane) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
     __syncwarp();
 }
-// The largest scales of a tile as bf16 bits: of its two groups, or of even and odd keys.
+// Whether a scale of the tile may be exactly 1.
 template <int HD>
-__device__ __forceinline__ void largest_scales(const uint8_t* vs, int lane, uint32_t& s0, uint32_t& s1) {
+__device__ __forceinline__ bool has_one(const uint8_t* vs, int lane) {
     constexpr int NG = HD / FORGE_KV4_GROUP;
-    uint32_t s = 0;
+    uint32_t w = 0xFFFFFFFFu;
 #pragma unroll
-    for (int k = 0; k < kKeys * NG / 2; k += 32)
-        if (k + lane < kKeys * NG / 2) s = __vmaxu2(s, reinterpret_cast<const uint32_t*>(vs)[k + lane] & 0x7FFF7FFFu);
-    s0 = __reduce_max_sync(0xffffffffu, s & 0xffffu);
-    s1 = __reduce_max_sync(0xffffffffu, s >> 16);
+    for (int k = 0; k < kKeys * NG / 2; k += 32) w = __vminu2(w, reinterpret_cast<const uint32_t*>(vs)[k + lane] ^ 0x3F803F80u);
+    return !(w & 0xffffu) || !(w >> 16);
 }
+// Makes the scales of a tile's groups of zeros 0: the format gives them 1, which would be the unit of the weights where
+// the other values are small. (Only a scale of exactly 1 has its codes looked at; other groups have a code of 0 or 14.)
+template <int HD>
+__device__ __forceinline__ void drop_zeros(bool one, uint8_t* vs, const uint8_t* vc, int lane) {
+    constexpr int NG = HD / FORGE_KV4_GROUP;
+    if (!__any_sync(0xffffffffu, one)) return;
+#pragma unroll 1
+    for (int e = lane; e < kKeys * NG; e += 32) {
+        uint16_t* s = reinterpret_cast<uint16_t*>(vs) + e;
+        if (*s != 0x3F80u) continue;
+        const uint4* c = reinterpret_cast<const uint4*>(vc + e / NG * (HD / 2) + e % NG * 32);
+        const uint4 a = c[0], b = c[1];
+        if ((a.x & a.y & a.z & a.w & b.x & b.y & b.z & b.w) == 0x77777777u && (a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) == 0x77777777u) *s = 0;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
+    __syncwarp();
+}
+// The bits of a weight, for the largest of a tile: negative or no number (a scale that is) above all others.
+__device__ __forceinline__ uint32_t larger(uint32_t m, F2 y) { return __vimax3_u32(m, __float_as_uint(y.x()), __float_as_uint(y.y())); }
+constexpr uint32_t kNoWeight = 0x7F800000u;  // from here on
+constexpr float kLeastUnit = 0x1p-100f;      // of a tile's largest weight (its inverse times 2^23 is an fp32 number)
 // A key's scales, both groups' or one's.
 template <int NG>
 __device__ __forceinline__ uint32_t scale_word(const uint8_t* base, int key) {
@@ -277,6 +299,7 @@ struct Many {
         uint8_t* vs = slot + 2 * Geo<HD>::kCodes + Geo<HD>::kScales;
         const uint8_t* krow = kc + (4 * (g >> 1) + (g & 1)) * (HD / 2) + 8 * t;  // this lane's keys of B, and of V's transposition
         const uint8_t* vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
+        const bool one = has_one<HD>(vs, lane);
         // ---- scores of keys 16 (u / 2) + 4 t + 2 (u % 2) + {0, 1}, head h, over fac
         F2 x[U];
 #pragma unroll
@@ -301,7 +324,7 @@ struct Many {
 #pragma unroll
         for (int u = 0; u < U; ++u)  // the other digits
             x[u] = x[u] + F2(__shfl_xor_sync(0xffffffffu, x[u].x(), 16), __shfl_xor_sync(0xffffffffu, x[u].y(), 16));
-        // ---- the tile's largest score and V scales; keys behind the last one count for nothing
+        // ---- the tile's largest score; keys behind the last one count for nothing
         if (left < kKeys) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -311,8 +334,7 @@ struct Many {
             }
             clear_scales<HD>(vs, left, lane);
         }
-        uint32_t smax0, smax1;
-        largest_scales<HD>(vs, lane, smax0, smax1);
+        drop_zeros<HD>(one, vs, kc + Geo<HD>::kCodes, lane);
         float mx = fmaxf(x[0].x(), x[0].y());
 #pragma unroll
         for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
@@ -339,21 +361,30 @@ struct Many {
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             // weights p sv unit < 2^23: 2^23 + weight has them in its low bits. (rcp is off by an ulp, the same for the tile)
-            const uint32_t sx = NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0;
-            const float smx = fmaxf(bf16_bits_to_f32((uint16_t)sx), 0x1p-100f), unit = rcp(smx) * (8388608.f * 255.f / 256.f);
-            const float wa = beta * smx * (256.f / 255.f / 8388608.f) * da, wb = beta * smx * (256.f / 255.f / 8388608.f) * db;
+            F2 y[U];
+            uint32_t big = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                y[u] = x[u] * sv[u / 2].of(u & 1, i);
+                big = larger(big, y[u]);
+            }
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const float ymx = fmaxf(__uint_as_float(big), kLeastUnit), unit = rcp(ymx) * (8388608.f * 255.f / 256.f);
+            const float back = big ? beta * ymx * (256.f / 255.f / 8388608.f) : 0.f;  // (rows of zeros give zeros)
+            const float wa = back * da, wb = back * db;
             const int4 magic = from[8 * NG];
             uint4 pa[U / 4];
             int c7[4];
 #pragma unroll
             for (int kb = 0; kb < U / 4; ++kb) {
-                uint32_t y[4];  // two digits of keys 32 kb + 16 (k / 2) + 4 t + 2 (k % 2) + {0, 1}
+                uint32_t w[4];  // two digits of keys 32 kb + 16 (k / 2) + 4 t + 2 (k % 2) + {0, 1}
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const F2 n = fma2(x[4 * kb + k], sv[2 * kb + k / 2].of(k & 1, i) * F2(unit, unit), F2(8388608.f, 8388608.f));
-                    y[k] = prmt(__float_as_uint(n.x()), __float_as_uint(n.y()), sel);
+                    const F2 n = fma2(y[4 * kb + k], F2(unit, unit), F2(8388608.f, 8388608.f));
+                    w[k] = prmt(__float_as_uint(n.x()), __float_as_uint(n.y()), sel);
                 }
-                pa[kb] = make_uint4(prmt(y[0], y[1], 0x5410), prmt(y[0], y[1], 0x7632), prmt(y[2], y[3], 0x5410), prmt(y[2], y[3], 0x7632));
+                pa[kb] = make_uint4(prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410), prmt(w[2], w[3], 0x7632));
                 mma_u8u8(c7, pa[kb], 0x07070707u, 0x07070707u, kb ? quad(c7) : magic);
             }
             // odd dims are 16 times; digit a's 7s and offset come off exactly, digit b's to below a unit of the weights
@@ -380,8 +411,8 @@ struct Many {
                     o[i][4 * j + n] = fma2(na, F2(ua, ua), fma2(float_bits(c[n][2], c[n][3]), F2(ub, ub), join));
                 }
             }
-            // (a scale that is no number has no digits)
-            if (sx >= 0x7F80u)
+            // (a scale that is negative or no number has no digits)
+            if (big >= kNoWeight)
 #pragma unroll
                 for (int n = 0; n < 8; ++n) o[i][n] = F2(NAN, NAN);
         }
@@ -499,6 +530,7 @@ struct Few {
         uint8_t* vs = slot + 2 * Geo<HD>::kCodes + Geo<HD>::kScales;
         const uint8_t *krow = kc + g * (HD / 2) + 8 * t, *vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
         const int4 magic = from[4 * NG];
+        const bool one = has_one<HD>(vs, lane);
         // ---- scores of keys 16 b + g and + 8, head h, over fac
         F2 x[kBlocks];
 #pragma unroll
@@ -520,15 +552,14 @@ struct Few {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)  // the other digits
             x[b] = x[b] + F2(__shfl_xor_sync(0xffffffffu, x[b].x(), 1), __shfl_xor_sync(0xffffffffu, x[b].y(), 1));
-        // ---- the tile's largest score and V scales; keys behind the last one count for nothing
+        // ---- the tile's largest score; keys behind the last one count for nothing
         if (left < kKeys) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
                 x[b] = F2(16 * b + g < left ? x[b].x() : -INFINITY, 16 * b + 8 + g < left ? x[b].y() : -INFINITY);
             clear_scales<HD>(vs, left, lane);
         }
-        uint32_t smax0, smax1;
-        largest_scales<HD>(vs, lane, smax0, smax1);
+        drop_zeros<HD>(one, vs, kc + Geo<HD>::kCodes, lane);
         float mx = fmaxf(x[0].x(), x[0].y());
 #pragma unroll
         for (int b = 1; b < kBlocks; ++b) mx = max3(mx, x[b].x(), x[b].y());
@@ -553,18 +584,23 @@ struct Few {
 
         // ---- weights p sv unit < 2^23, added to 2^23, of head h: lane t of the two for group t % 2 (both the same where there
         // is one); through shared memory to the lanes whose column needs their keys
-        float smx[NG];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) smx[i] = fmaxf(bf16_bits_to_f32((uint16_t)(NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0)), 0x1p-100f);
+        uint32_t mine = 0;  // the largest of this lane's group
         {
             const int i = NG == 2 ? t & 1 : 0;
-            const float unit = rcp(NG == 2 && i ? smx[NG - 1] : smx[0]) * (8388608.f * 255.f / 256.f);  // (off by an ulp, the same for the tile)
-            uint32_t* y = ys + (h * NG + i) * kRowY + g;
             const uint16_t* sv = reinterpret_cast<const uint16_t*>(vs) + g * NG + i;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-                const F2 s2(bf16_bits_to_f32(sv[16 * b * NG]), bf16_bits_to_f32(sv[(16 * b + 8) * NG]));
-                const F2 n = fma2(x[b], s2 * F2(unit, unit), F2(8388608.f, 8388608.f));
+                x[b] = x[b] * F2(bf16_bits_to_f32(sv[16 * b * NG]), bf16_bits_to_f32(sv[(16 * b + 8) * NG]));
+                mine = larger(mine, x[b]);
+            }
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 8));
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 16));
+            const float unit = rcp(fmaxf(__uint_as_float(mine), kLeastUnit)) * (8388608.f * 255.f / 256.f);  // (off by an ulp, the same for the tile)
+            uint32_t* y = ys + (h * NG + i) * kRowY + g;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const F2 n = fma2(x[b], F2(unit, unit), F2(8388608.f, 8388608.f));
                 y[16 * b] = __float_as_uint(n.x());
                 y[16 * b + 8] = __float_as_uint(n.y());
             }
@@ -574,7 +610,9 @@ struct Few {
         // ---- O += P V, group by group
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            const float wa = beta * smx[i] * (256.f / 255.f / 8388608.f) * da, wb = beta * smx[i] * (256.f / 255.f / 8388608.f) * db;
+            const uint32_t big = __shfl_sync(0xffffffffu, mine, (lane & ~1) | i);
+            const float back = big ? beta * fmaxf(__uint_as_float(big), kLeastUnit) * (256.f / 255.f / 8388608.f) : 0.f;  // (rows of zeros give zeros)
+            const float wa = back * da, wb = back * db;
             uint2 pb[kKeys / 32];
             int c7[4];
 #pragma unroll
@@ -605,8 +643,8 @@ struct Few {
                     at = fma2(na, F2(ua, ua), fma2(nb, F2(ub, ub), at * F2(alpha, alpha)));
                 }
             }
-            // (a scale that is no number has no digits)
-            if ((NG == 1 ? max(smax0, smax1) : i ? smax1 : smax0) >= 0x7F80u)
+            // (a scale that is negative or no number has no digits)
+            if (big >= kNoWeight)
 #pragma unroll
                 for (int n = 0; n < 4; ++n) o[i][n] = F2(NAN, NAN);
         }

@@ -64,8 +64,13 @@ int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos
  * over positions 0..pos[b] of sequence seq[b] (seq NULL: sequence b), query
  * head h reading KV head h / (H / n_kv_head). q and out [B][H * head_dim]
  * fp32, 16-byte aligned; H a multiple of n_kv_head; scores, softmax and sums
- * in fp32 (the products on the tensor cores in integers, exactly: q and the
- * weights of 64 keys rounded to 23 bits of their largest). pos[b] < 0: an
+ * in fp32. The products are on the tensor cores in integers, exactly: q is
+ * rounded to 23 bits of its head's largest channel, and the weights (a key's
+ * probability times its V's scale) of 64 keys to 23 bits of their largest for a
+ * head and group of 64 dims, so an output's error is relative to the sum of the
+ * weighted rows' largest values in the group (or to 2^-100 where that is less).
+ * A scale of V that is NaN or negative, which append does not write, makes the
+ * group's output NaN. pos[b] < 0: an
  * empty sequence, its output is zeros (a padded batch). A position beyond the
  * cache, or a page outside the pool, sets the error word and makes the
  * sequence's output NaN.

@@ -143,6 +143,13 @@ __device__ __forceinline__ bool elect_one() {
     return p;
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// The scores' integer sums (below 2^32 for q's below 2^e) are taken down by this power of two, so that no scale of K takes
+// them out of fp32's range; not for q's so large that a large scale would take the score itself out.
+__device__ __forceinline__ int sum_down(int e) { return e <= 64 ? 32 : 0; }
+// Factors of a lane's two sums that start at 1.5 2^23, and what takes that off.
+__device__ __forceinline__ int4 factors(float a, float b) {
+    return make_int4(__float_as_int(a), __float_as_int(b), __float_as_int(-12582912.f * (a + b)), 0);
+}
 __device__ __forceinline__ F2 float_bits(int x, int y) { return F2(__int_as_float(x), __int_as_float(y)); }
 
 // Tiles of sequence slot b; -1 when its position or sequence is out of range.
@@ -224,9 +231,9 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* base, int key) {
 template <int HD>
 struct Many {
     static constexpr int kHeads = kHeadsMany, kCtas = kCtasMany, NG = HD / FORGE_KV4_GROUP, U = kKeys / 8;
-    static constexpr int kSmem = 2 * NG * 512 + NG * 128 + 16;  // A operands of q [2 groups][32 lanes], sums to start from [groups][8], kMagic
+    static constexpr int kSmem = 2 * NG * 512 + NG * 128 + 16 + 128;  // A operands of q [2 groups][32 lanes], sums to start from [groups][8], kMagic, factors [8]
     const int warp, lane, g, t, h;
-    const float da, db, off;  // this lane's rows: digit a (2 or 1) and digit b (0, or none) of head h
+    const float da, db;       // this lane's rows: digit a (2 or 1) and digit b (0, or none) of head h
     const uint32_t sel;       // digits a of two words, then digits b
     uint4* qs;
     int4* from;
@@ -235,7 +242,7 @@ struct Many {
 
     __device__ Many(uint8_t* smem, int warp, int lane)
         : warp(warp), lane(lane), g(lane >> 2), t(lane & 3), h(g & 3), da(g < 4 ? 65536.f : 256.f), db(g < 4 ? 1.f : 0.f),
-          off(-12582912.f * (da + db)), sel(g < 4 ? 0x4062 : 0xBB51), qs(reinterpret_cast<uint4*>(smem)),
+          sel(g < 4 ? 0x4062 : 0xBB51), qs(reinterpret_cast<uint4*>(smem)),
           from(reinterpret_cast<int4*>(smem + 2 * NG * 512)) {
         if (threadIdx.x == 0) from[8 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
     }
@@ -257,9 +264,11 @@ struct Many {
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
-        const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
-        const float up = pow2i(23 - e);
-        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
+        const int e = (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126, sd = sum_down(e);
+        const float up = pow2i(min(23 - e, 127)), up2 = pow2i(max(23 - e, 127) - 127);  // (for the smallest q, two factors)
+        const float down = pow2i(-sd);
+        if (warp == 0 && t == 0) from[8 * NG + 1 + g] = factors(da * down, db * down);
+        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23 + sd);  // (an infinite or NaN q: all NaN)
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             int sa = 0, sb = 0;
@@ -270,7 +279,7 @@ struct Many {
                 uint32_t da[8], db[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
+                    const int n = __float2int_rn(x[k] * up * up2), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
                     da[k] = g < 4 ? (n1 - d1) >> 8 : d1;
                     db[k] = g < 4 ? d0 : 0;
                 }
@@ -300,6 +309,8 @@ struct Many {
         const uint8_t* krow = kc + (4 * (g >> 1) + (g & 1)) * (HD / 2) + 8 * t;  // this lane's keys of B, and of V's transposition
         const uint8_t* vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
         const bool one = has_one<HD>(vs, lane);
+        const int4 fs = from[8 * NG + 1 + g];
+        const float sa = __int_as_float(fs.x), sb = __int_as_float(fs.y), off = __int_as_float(fs.z);
         // ---- scores of keys 16 (u / 2) + 4 t + 2 (u % 2) + {0, 1}, head h, over fac
         F2 x[U];
 #pragma unroll
@@ -315,8 +326,8 @@ struct Many {
                     int c[4];
                     mma_s8u8(c, q0, even(w.x), even(w.x >> 4), c0);
                     mma_s8u8(c, q1, even(w.y), even(w.y >> 4), quad(c));
-                    // digit a times da + digit b times db; both offsets of 12582912 come off exactly with the first
-                    const F2 sum = fma2(float_bits(c[2], c[3]), F2(db, db), fma2(float_bits(c[0], c[1]), F2(da, da), F2(off, off)));
+                    // digit a times sa + digit b times sb; both offsets of 12582912 come off exactly with the first
+                    const F2 sum = fma2(float_bits(c[2], c[3]), F2(sb, sb), fma2(float_bits(c[0], c[1]), F2(sa, sa), F2(off, off)));
                     x[u0 + f] = i ? fma2(sum, sk.of(f, i), x[u0 + f]) : sum * sk.of(f, i);
                 }
             }
@@ -457,9 +468,9 @@ struct Few {
     static constexpr int kHeads = kHeadsFew, kCtas = kCtasFew, NG = HD / FORGE_KV4_GROUP, kBlocks = kKeys / 16;
     static constexpr int kRowY = kKeys + 8;                              // words of a (head, group)'s weights, no bank twice
     static constexpr int kY = kHeads * NG * kRowY * 4;                   // a warp's weights
-    static constexpr int kSmem = NG * 64 + 16 + kWarps * kY;             // sums to start from [groups][t], kMagic, weights
+    static constexpr int kSmem = NG * 64 + 16 + 64 + kWarps * kY;        // sums to start from [groups][t], kMagic, factors [t], weights
     const int warp, lane, g, t, h, hq;
-    const float da, db, off;  // this lane's columns 2 t, 2 t + 1: digits 2 and 1 of head h, or digit 0 and nothing
+    const float da, db;       // this lane's columns 2 t, 2 t + 1: digits 2 and 1 of head h, or digit 0 and nothing
     const uint32_t sel;       // the digit of column g, of two words
     int4* from;
     uint32_t* ys;
@@ -469,9 +480,9 @@ struct Few {
 
     __device__ Few(uint8_t* smem, int warp, int lane)
         : warp(warp), lane(lane), g(lane >> 2), t(lane & 3), h(t >> 1), hq(g >> 2), da(t & 1 ? 1.f : 65536.f),
-          db(t & 1 ? 0.f : 256.f), off(-12582912.f * (da + db)),
+          db(t & 1 ? 0.f : 256.f),
           sel((g & 3) == 0 ? 0x62 : (g & 3) == 1 ? 0x51 : (g & 3) == 2 ? 0x40 : 0xFB), from(reinterpret_cast<int4*>(smem)),
-          ys(reinterpret_cast<uint32_t*>(smem + NG * 64 + 16 + warp * kY)) {
+          ys(reinterpret_cast<uint32_t*>(smem + NG * 64 + 16 + 64 + warp * kY)) {
         if (threadIdx.x == 0) from[4 * NG] = make_int4(kMagic, kMagic, kMagic, kMagic);
     }
     __device__ int q_head() const { return hq; }
@@ -492,9 +503,11 @@ struct Few {
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         // 2^e > 1.004 |q|: |q| 2^(23 - e) is at most 127 (1 + 2^8 + 2^16), the largest three signed digits
-        const int e = max(-100, (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126);
-        const float up = pow2i(23 - e);
-        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23);  // (an infinite or NaN q: all NaN)
+        const int e = (int)(__float_as_uint(1.004f * __uint_as_float(mx)) >> 23) - 126, sd = sum_down(e);
+        const float up = pow2i(min(23 - e, 127)), up2 = pow2i(max(23 - e, 127) - 127);  // (for the smallest q, two factors)
+        const float down = pow2i(-__shfl_sync(0xffffffffu, sd, 16 * h));
+        if (warp == 0 && g == 0) from[4 * NG + 1 + t] = factors(da * down, db * down);
+        fac = mx >= 0x7F800000u ? NAN : scale_log2 * pow2i(e - 23 + sd);  // (an infinite or NaN q: all NaN)
         fac = __shfl_sync(0xffffffffu, fac, 16 * h);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -506,7 +519,7 @@ struct Few {
                 uint32_t d[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int n = __float2int_rn(x[k] * up), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
+                    const int n = __float2int_rn(x[k] * up * up2), d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1;
                     d[k] = (g & 3) == 0 ? (n1 - d1) >> 8 : (g & 3) == 1 ? d1 : (g & 3) == 2 ? d0 : 0;
                 }
                 qb[i][w] = make_uint2(low_bytes(d), low_bytes(d + 4));
@@ -531,6 +544,8 @@ struct Few {
         const uint8_t *krow = kc + g * (HD / 2) + 8 * t, *vrow = kc + Geo<HD>::kCodes + lane * (HD / 2);
         const int4 magic = from[4 * NG];
         const bool one = has_one<HD>(vs, lane);
+        const int4 fs = from[4 * NG + 1 + t];
+        const float sa = __int_as_float(fs.x), sb = __int_as_float(fs.y), off = __int_as_float(fs.z);
         // ---- scores of keys 16 b + g and + 8, head h, over fac
         F2 x[kBlocks];
 #pragma unroll
@@ -543,8 +558,8 @@ struct Few {
                 int c[4];
                 mma_u8s8(c, make_uint4(even(w.x), even(z.x), even(w.x >> 4), even(z.x >> 4)), qb[i][0].x, qb[i][0].y, from[4 * i + t]);
                 mma_u8s8(c, make_uint4(even(w.y), even(z.y), even(w.y >> 4), even(z.y >> 4)), qb[i][1].x, qb[i][1].y, quad(c));
-                // digits times da and db; both offsets of 12582912 come off exactly with the first
-                const F2 sum = fma2(float_bits(c[1], c[3]), F2(db, db), fma2(float_bits(c[0], c[2]), F2(da, da), F2(off, off)));
+                // digits times sa and sb; both offsets of 12582912 come off exactly with the first
+                const F2 sum = fma2(float_bits(c[1], c[3]), F2(sb, sb), fma2(float_bits(c[0], c[2]), F2(sa, sa), F2(off, off)));
                 const F2 sp = i ? F2(bf16_hi_f32(s0), bf16_hi_f32(s1)) : F2(bf16_lo_f32(s0), bf16_lo_f32(s1));
                 x[b] = i ? fma2(sum, sp, x[b]) : sum * sp;
             }

@@ -160,3 +160,22 @@ def test_decode_at_every_boundary(forge, cuda, hd, H, Hkv, page):
     got = kv4.decode(forge, cuda, cache, q, pos)
     forge.check(forge.lib().forge_ops_check(), "error word")
     kv4.check(got, reference(cache, q, pos))
+
+
+@pytest.mark.parametrize("hd,H,Hkv", [(128, 2, 2), (64, 2, 1), (128, 8, 2), (64, 4, 1)])
+def test_decode_of_extreme_sizes(forge, cuda, hd, H, Hkv):
+    """Scores of ordinary size from tiny queries and huge keys and the other way round, up to the ends of fp32 and bf16;
+    V at the ends as well."""
+    sizes = [(1e-30, 1e30, 1.0), (1e-37, 1e37, 1.0), (1e37, 1e-37, 1.0), (1e20, 1e-20, 1e37), (1e18, 1e-18, 1e-25),
+             (1e-18, 1e20, 1.0), (1e36, 1e-30, 1.0), (1.0, 1.0, 1e37)]
+    n = 150
+    rng = np.random.default_rng(hd + H)
+    cache = kv4.Cache(forge, cuda, len(sizes), Hkv, hd, 152, 0, seed=7)
+    q = rng.standard_normal((len(sizes), H, hd)).astype(np.float32)
+    for b, (sq, sk, sv) in enumerate(sizes):
+        q[b] *= np.float32(sq)
+        for kv, f in ((0, sk), (1, sv)):
+            cache.scales[kv][b] = kv4.bf16((cache.scales[kv][b].astype(np.float64) * f).astype(np.float32))
+    upload(cache)
+    pos = [n - 1] * len(sizes)
+    kv4.check(kv4.decode(forge, cuda, cache, q, pos), reference(cache, q, pos))

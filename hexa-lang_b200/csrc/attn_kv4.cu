@@ -215,6 +215,9 @@ __device__ __forceinline__ void drop_zeros(bool one, uint8_t* vs, const uint8_t*
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the copies that come into the slot)
     __syncwarp();
 }
+// Scores (times log2 e) beyond this are taken relative to the tile's largest before they are multiplied: rounded, that is
+// steps of 2 and more off, and the largest p would be as far below 1, or 0.
+constexpr float kFar = 0x1p24f;
 // The bits of a weight, for the largest of a tile: negative or no number (a scale that is) above all others.
 __device__ __forceinline__ uint32_t larger(uint32_t m, F2 y) { return __vimax3_u32(m, __float_as_uint(y.x()), __float_as_uint(y.y())); }
 constexpr uint32_t kNoWeight = 0x7F800000u;  // from here on
@@ -351,9 +354,15 @@ struct Many {
         for (int u = 1; u < U; ++u) mx = max3(mx, x[u].x(), x[u].y());
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float top = mx;
         mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
         // p = 2^(x - mx) <= 1
-        const float nmx = mx == -INFINITY ? 0.f : -mx;
+        float nmx = mx == -INFINITY ? 0.f : -mx;
+        if (fabsf(mx) > kFar && fabsf(mx) < INFINITY) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = x[u] + F2(-top, -top);
+            nmx = 0.f;
+        }
         F2 ls;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -581,9 +590,15 @@ struct Few {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float top = mx;
         mx = __fmul_ru(mx, fac);  // (up, so that no difference to it comes out above 0)
         // p = 2^(x - mx) <= 1
-        const float nmx = mx == -INFINITY ? 0.f : -mx;
+        float nmx = mx == -INFINITY ? 0.f : -mx;
+        if (fabsf(mx) > kFar && fabsf(mx) < INFINITY) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) x[b] = x[b] + F2(-top, -top);
+            nmx = 0.f;
+        }
         F2 ls;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {

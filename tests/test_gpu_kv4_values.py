@@ -179,3 +179,37 @@ def test_decode_of_extreme_sizes(forge, cuda, hd, H, Hkv):
     upload(cache)
     pos = [n - 1] * len(sizes)
     kv4.check(kv4.decode(forge, cuda, cache, q, pos), reference(cache, q, pos))
+
+
+@pytest.mark.parametrize("hd,H,Hkv", [(128, 2, 2), (64, 2, 1), (128, 8, 2), (64, 4, 1)])
+def test_decode_of_far_scores(forge, cuda, hd, H, Hkv):
+    """Scores from 1e8 to 1e30 of both signs: the key with the largest has all the weight, wherever it lies. (The gap to
+    the next is above a score's error, so the others' weights are below 2^-100; what is left is the rounding of one
+    weight, one sum and one quotient: 8 u.)"""
+    n, sizes = 200, [1e4, 3e4, 1e5, 1e7, 1e15]
+    rng = np.random.default_rng(hd + H)
+    cache = kv4.Cache(forge, cuda, 2 * len(sizes), Hkv, hd, 200, 0, seed=8)
+    sign = np.where(rng.random((Hkv, hd)) < 0.5, -0.5, 0.5)
+    q = np.repeat(sign, H // Hkv, 0)[None].repeat(2 * len(sizes), 0)
+    top = rng.integers(0, n, 2 * len(sizes))
+    for b in range(2 * len(sizes)):
+        size, below = sizes[b // 2], b % 2
+        k = size * sign * rng.uniform(0.1, 0.8, (n, Hkv, 1))
+        k[top[b]] = size * sign * 0.9
+        if below:  # all of them negative, the smallest in size on top
+            k = size * sign - k
+        fill(cache, b, 0, k * (-1 if below else 1))
+        q[b] *= size
+    upload(cache)
+    q = q.astype(np.float32)
+    pos = [n - 1] * len(q)
+    got = kv4.decode(forge, cuda, cache, q, pos)
+    for b in range(len(q)):
+        k, v = (cache.row(kv, b, n) for kv in range(2))
+        for h in range(H):
+            g = h // (H // Hkv)
+            s = k[:, g] @ q[b, h].astype(np.float64) / np.sqrt(hd)
+            ds = 10 * U * (np.abs(k[:, g]) @ np.abs(q[b, h].astype(np.float64))).max() / np.sqrt(hd)
+            assert s[top[b]] - np.delete(s, top[b]).max() > 100 + 2 * ds and (s.max() < 0) == bool(b % 2)
+            vmax = np.repeat(np.abs(v[top[b], g]).reshape(-1, 64).max(-1), 64)
+            assert (np.abs(got[b, h] - v[top[b], g]) <= 8 * U * vmax).all(), (b, h)

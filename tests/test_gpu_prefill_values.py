@@ -1,0 +1,42 @@
+"""The packed prefill's fp32 statistics and its edges, with inputs whose
+scores are known exactly."""
+import numpy as np
+import pytest
+
+import test_gpu_prefill_varlen as pv
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -23
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(2, 1), (3, 3)])
+def test_lse_to_fp32(forge, cuda, hd, H, Hkv):
+    """Rows of up to 64 keys whose scores are products of one channel, exact in fp32: key 0 at 0, every eighth of the
+    others at -d, the rest at -400 (no weight). With |x| = d log2 e below 3.7, the factor's and the exponent's roundings
+    are 2.6 u of a probability and its exp2 is off by 2 u; a sum has 9 terms that are not 0, 4.5 u; the logarithm, its
+    factor and their product 2 u |lse|."""
+    import torch
+    lens, w = 64, hd * (H + 2 * Hkv)
+    d = torch.linspace(0, 2.5, 161).mul(hd ** 0.5).to(torch.bfloat16)  # a sequence each
+    n = len(d)
+    x = torch.zeros(n, lens, w, dtype=torch.bfloat16)
+    x[:, :, 0:H * hd:hd] = 1
+    keys = torch.full((8, n, lens), -400.0 * hd ** 0.5).to(torch.bfloat16)
+    keys[:, :, 0] = 0
+    for part in range(8):
+        keys[part, :, part::8] = -d[:, None]
+        keys[part, :, 0] = 0
+    for part in range(8):
+        x[:, :, H * hd:(H + Hkv) * hd:hd] = keys[part][:, :, None]
+        rows = x.view(n * lens, w).to(cuda)
+        q, k, v = rows[:, :H * hd], rows[:, H * hd:(H + Hkv) * hd], rows[:, (H + Hkv) * hd:]
+        o = torch.full((n * lens, H * hd), float("nan"), dtype=torch.bfloat16, device=cuda)
+        lse = torch.full((H, n * lens), float("nan"), device=cuda)
+        pv.run(forge, cuda, q, k, v, [lens * i for i in range(n + 1)], H, Hkv, hd, o, lse)
+        forge.check(forge.lib().forge_ops_check(), "error word")
+        s = keys[part].double() / hd ** 0.5                      # [n][64]
+        hide = torch.ones(lens, lens, dtype=torch.bool).triu(1)
+        want = torch.logsumexp(s[:, None, :].masked_fill(hide, float("-inf")), -1).flatten()
+        err = (lse.double().cpu() - want).abs()
+        assert (err <= U * (9.1 + 2 * want.abs())).all(), (part, (err / U).max().item())

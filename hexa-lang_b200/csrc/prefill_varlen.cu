@@ -60,6 +60,7 @@ constexpr int kThreads = 352;
 constexpr int kMaxCtas = 160;  // (5 loads per lane of the items warp)
 constexpr int kItemCost = 1;   // what an item costs beside its key blocks, in blocks
 constexpr int kSlots = 5;      // K/V ring
+constexpr int kMostOverlap = 4;  // how often the sequences may name a row, on average
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kIdescS = umma_idesc_bf16_f32(kBM, kSub, false);
 template <int HD> constexpr int tile_bytes() { return kBM * HD * 2; }
@@ -121,18 +122,27 @@ struct Dealer {
     int load[kMaxCtas / 32];  // of CTAs lane, lane + 32, ...
     int next, last;         // this CTA's items [next, last) of depth p
 
-    __device__ int depth(int s) const {  // of sequence s, in tiles; none where its bounds are bad
+    __device__ int length(int s) const {  // of sequence s; 0 where its bounds are bad
         if (s >= a.n_seq) return 0;
         const int b = a.cu[s], e = a.cu[s + 1];
-        return b < 0 || e < b || e > a.total ? 0 : (e - b + rows - 1) / rows;
+        return b < 0 || e < b || e > a.total ? 0 : e - b;
     }
+    __device__ int depth(int s) const { return (length(s) + rows - 1) / rows; }  // in tiles
     __device__ explicit Dealer(const VarlenArgs& args) : a(args) {}
     __device__ void start() {
         rows = a.pair_heads ? kBM : 2 * kBM;
         heads = a.pair_heads ? a.H / 2 : a.H;
         int most = 0;
-        for (int s0 = 0; s0 < a.n_seq; s0 += 32) most = max(most, depth(s0 + (threadIdx.x & 31)));
+        unsigned whole = 0;  // whole tiles of 128 rows
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+            const int n = length(s0 + (threadIdx.x & 31));
+            most = max(most, (n + rows - 1) / rows);
+            whole = min(whole + n / kBM, 1u << 26);  // (no overflow of the warp's sum)
+        }
         deepest = (int)__reduce_max_sync(0xffffffffu, most);
+        // Bounds that decrease can name the rows many times over, more work than any packing of them: nothing is done.
+        // (Of sequences that do not overlap, the whole tiles are at most total / 128, which is below 2^23.)
+        if (__reduce_add_sync(0xffffffffu, whole) > (unsigned)kMostOverlap * (a.total / kBM + 1)) deepest = 0;
         group = a.group;
         p = deepest;
         h0 = 0;

@@ -338,7 +338,8 @@ int forge_flash_prefill(const uint16_t* q, const uint16_t* k, const uint16_t* v,
  * Rows before cu_seqlens[0] and from cu_seqlens[n_seq] on are not written. A
  * sequence whose bounds decrease or leave 0..total sets the error word
  * (forge_ops_check) and is left out (rows that two of the others then share
- * hold either's result). A NaN or infinity in k or v reaches its
+ * hold either's result; where the others add up to more than about four times
+ * total, all are left out). A NaN or infinity in k or v reaches its
  * own sequence's rows only, there possibly rows up to 127 before it. Arrays
  * 16-byte aligned, row lengths multiples of 8 elements; o must not overlap
  * the inputs. Asynchronous on stream. */

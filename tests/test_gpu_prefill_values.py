@@ -40,3 +40,27 @@ def test_lse_to_fp32(forge, cuda, hd, H, Hkv):
         want = torch.logsumexp(s[:, None, :].masked_fill(hide, float("-inf")), -1).flatten()
         err = (lse.double().cpu() - want).abs()
         assert (err <= U * (9.1 + 2 * want.abs())).all(), (part, (err / U).max().item())
+
+
+@pytest.mark.parametrize("H,Hkv", [(4, 1), (3, 3)])
+def test_bounds_that_name_rows_many_times(forge, cuda, H, Hkv):
+    """cu_seqlens that goes up and down again: the error word is set, and where the rows would be computed many times
+    over nothing is; twice over is answered. Zero lengths and short prompts in number are no overlap."""
+    import torch
+    total, hd = 600, 64
+    q, k, v = pv.make(torch, cuda, total, H, Hkv, hd, seed=1)
+    for n, left_out in ((2, False), (40, True), (3000, True)):
+        o = torch.full((total, H * hd), 9.0, dtype=torch.bfloat16, device=cuda)
+        pv.run(forge, cuda, q, k, v, [0, total] * n, H, Hkv, hd, o, None)
+        with pytest.raises(forge.ForgeError, match="error word"):
+            forge.check(forge.lib().forge_ops_check(), "error word")
+        if left_out:
+            assert (o == 9).all()
+        else:
+            pv.check(torch, q, k, v, [0, total], H, Hkv, hd, o, None)
+    for lens in ([1] * 600, [0, 1, 0] * 200 + [0] * 500 + [400], [600] + [0] * 3000):
+        cu = [0] + np.cumsum(lens).tolist()
+        o = torch.full((total, H * hd), float("nan"), dtype=torch.bfloat16, device=cuda)
+        pv.run(forge, cuda, q, k, v, cu, H, Hkv, hd, o, None)
+        forge.check(forge.lib().forge_ops_check(), "error word")
+        pv.check(torch, q, k, v, cu, H, Hkv, hd, o, None)

@@ -60,6 +60,10 @@ constexpr int kThreads = 352;
 constexpr int kMaxCtas = 160;  // (5 loads per lane of the items warp)
 constexpr int kItemCost = 1;   // what an item costs beside its key blocks, in blocks
 constexpr int kSlots = 5;      // K/V ring
+// Where a row's maximum score times c = log2(e) / sqrt(hd) is beyond kFar, its rounding is a step of 64 and more, and the
+// largest P would be anything. Two scores that differ do so by 2^9 there, and the smaller has no weight, with c or with
+// the power of two next to it, whose product with the maximum is exact.
+constexpr float kFar = 0x1p30f, kFarScale = 0.125f;
 constexpr int kMostOverlap = 4;  // how often the sequences may name a row, on average
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kIdescS = umma_idesc_bf16_f32(kBM, kSub, false);
@@ -531,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int nmine = steps(it, t), qt = it.tile[t];
             // Running max in log2 units (m = max * c), raised only when a new score exceeds it by more than 8 (P stays
             // below 2^8, exact enough in bf16 and fp32), so O in TMEM is rescaled rarely; l and O refer to the same m.
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, cr = c, nm = 0.f;  // P = 2^(S cr + nm)
             bool ok = nmine > 0;
             for (int j = 0; j < nmine; ++j, np += j < nmine) {  // (the last P V has a barrier of its own)
                 const int buf = j & 1;
@@ -558,11 +562,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
                         mx4[(i >> 1) & 3] = max3_nan(mx4[(i >> 1) & 3], __uint_as_float(sv[q][i]), __uint_as_float(sv[q][i + 1]));
-                const float mxc = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
+                const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]), mxc = mx * c;
                 const bool raise = mxc > m + 8.0f || j == 0;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float alpha = raise && j > 0 ? ex2(m - mxc) : 1.0f;
-                    m = raise ? mxc : m;
+                    if (raise) {
+                        m = mxc;
+                        cr = fabsf(m) > kFar ? kFarScale : c;
+                        nm = fabsf(m) > kFar ? -kFarScale * mx : -m;
+                    }
                     l *= alpha;
                     if (j > 0) {
                         // P V of the step before has to be in O
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const F2 c2(c, c), nm2(-m, -m);
+                const F2 c2(cr, cr), nm2(nm, nm);
                 F2 sum(0.f, 0.f);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {

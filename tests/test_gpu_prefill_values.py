@@ -64,3 +64,33 @@ def test_bounds_that_name_rows_many_times(forge, cuda, H, Hkv):
         pv.run(forge, cuda, q, k, v, cu, H, Hkv, hd, o, None)
         forge.check(forge.lib().forge_ops_check(), "error word")
         pv.check(torch, q, k, v, cu, H, Hkv, hd, o, None)
+
+
+@pytest.mark.parametrize("hd,H,Hkv", [(64, 4, 2), (128, 2, 1), (128, 3, 3)])
+@pytest.mark.parametrize("below", [False, True])
+def test_far_scores(forge, cuda, hd, H, Hkv, below):
+    """Scores from 1e8 to 1e30 of both signs, the largest so far replaced now and then: its key has all the weight (the
+    others' are below 2^-1000), so the output is its row of V and the LSE its score to three roundings. The key's P is
+    2^r, r the rounding of its score, not 1: as a bf16 off by 2^-8 of itself, while the sum has it in fp32; the output is
+    rounded by 2^-8 as well. Both together 2.01 2^-8 |v|."""
+    import torch
+    n = 330
+    rng = np.random.default_rng(5)
+    val = rng.uniform(0.1, 0.4, n)
+    for j, r in zip((0, 5, 63, 64, 127, 130, 200, 329), np.linspace(0.5, 0.95, 8)):
+        val[j] = r
+    best = np.maximum.accumulate(np.where(val >= 0.5, np.arange(n), 0))
+    for size in (1e4, 1e5, 1e6, 1e8, 1e15):
+        q, k, v = pv.make(torch, cuda, n, H, Hkv, hd, seed=2)
+        q.zero_(), k.zero_()
+        q[:, ::hd] = size
+        k[:, ::hd] = torch.tensor((val - below) * size).to(torch.bfloat16).to(cuda)[:, None]
+        o = torch.full((n, H * hd), float("nan"), dtype=torch.bfloat16, device=cuda)
+        lse = torch.full((H, n), float("nan"), device=cuda)
+        pv.run(forge, cuda, q, k, v, [0, n], H, Hkv, hd, o, lse)
+        forge.check(forge.lib().forge_ops_check(), "error word")
+        want = v.reshape(n, Hkv, hd).repeat_interleave(H // Hkv, 1)[best].flatten(1)
+        assert ((o.double() - want.double()).abs() <= 2.01 * 2.0 ** -8 * want.double().abs()).all(), size
+        s = k.reshape(n, Hkv, hd)[best, :, 0].double() * float(q[0, 0]) / hd ** 0.5
+        s = s.repeat_interleave(H // Hkv, 1).t()
+        assert ((lse.double() - s).abs() <= 2 * U * s.abs()).all(), size

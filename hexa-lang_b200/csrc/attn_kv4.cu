@@ -24,18 +24,21 @@
 //
 // Two forms, for how many query heads read a KV head. Up to 2: keys and dims
 // are the 16 rows of A and the digits of both heads 6 of the 8 columns, so a lane
-// has half of a tile's scores, exponentials and sums of the other form: 760
+// has half of a tile's scores, exponentials and sums of the other form: 800
 // instructions for 64 keys of 128 dims (pairs' starts and joins among them), and
-// 165 registers let 3 CTAs share an SM. 3 and more: 4 heads' digits are 12 of
-// the 16 rows, keys and dims the 8 columns: 845 instructions, fewer than two
-// passes of the first form, and the keys are read once for the 4. Measured, 64 sequences of 4096 with 40 heads
-// of 128, each reading its own KV head (1.43 GB; 218 us at the rate of a copy):
-// 220 us in the first form, 6.5 TB/s, bound by HBM, next by shared-memory banks
-// (0.74 of the wavefronts: ldmatrix's rows 64 bytes apart share them); 265 in the
-// second, bound by issue and latencies (0.49 of the issue slots with 2 warps a
-// scheduler; 3 would have 168 registers and spill). The same products in fp16, q and
-// weights as pairs of fp16, took 379. Short contexts are a chain of latencies:
-// 10 us for one sequence of 2048.
+// 168 registers let 3 CTAs share an SM. 3 and more: 4 heads' digits are 12 of
+// the 16 rows, keys and dims the 8 columns: 980 instructions (pages of 32), fewer
+// than two passes of the first form, and the keys are read once for the 4.
+// Measured, 64 sequences of 4096 with 40 heads of 128, each reading its own KV head
+// (1.43 GB; 218 us at the rate of a copy): 222 us in the first form, 6.4 TB/s,
+// bound by HBM, next by shared-memory banks (0.74 of the wavefronts: ldmatrix's
+// rows 64 bytes apart share them), 259 with 2 CTAs an SM; 280 in the second, bound by
+// issue and latencies (0.41 of the issue slots with 2 warps a scheduler; 3 would
+// have 168 registers and spill). 32 ragged sequences up to 16384, 4 heads a KV head:
+// 29.7 us in the second form, 37.5 in the first. The same products in fp16, q and
+// weights as pairs of fp16, took 379 for the former. Short contexts are a chain of
+// latencies: 10 us for one sequence of 2048. The unit of the weights costs 2 to 4%:
+// without it (see O) 217 and 28.2 us.
 //
 // Work: the tiles of 64 keys of all (sequence, KV head, heads of a pass) form
 // one line, every pair's tiles behind a few units for what a pair costs by
@@ -59,7 +62,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 64;          // keys per tile
 constexpr int kStages = 2;         // tiles a warp has in flight
 constexpr int kCtasMany = 2, kCtasFew = 3;  // CTAs per SM
-constexpr int kPairUnits = 6;      // what a pair costs beside its tiles, in tiles (4: 29.3 us for 32 ragged sequences, 6: 28.3)
+constexpr int kPairUnits = 6;      // what a pair costs beside its tiles, in tiles (4: 30.5 us for 32 ragged sequences, 6: 29.7)
 constexpr int kMinUnits = 2 * kWarps;  // least range of a CTA
 constexpr int kJoin = kWarps / 2;  // sums of warps that shared memory holds at the end of a pair
 constexpr int kHeadsMany = 4, kHeadsFew = 2;  // query heads that share a pass over the keys

@@ -13,7 +13,7 @@
 // deepest, its items raise the CTAs' loads to a common level.
 // Heads are dealt a group at a time, as many as keep their K and V in half of
 // L2 (for 8 prompts of 4096 with 32 KV heads all heads at once read HBM 2.6
-// times and took 1.11 ms instead of 0.99). Every CTA works this out for
+// times and took 1.12 ms instead of 1.01). Every CTA works this out for
 // itself, in a warp of its own that runs ahead of the others, so that any mix
 // of lengths is even without a table, a counter or a second launch (dealing
 // the sorted items out back and forth instead took up to 1.4 times as long).
@@ -29,15 +29,18 @@
 // O += P V. With two buffers the tensor cores run S of the next half block
 // while the exponentials of this one run: a tile's softmax never waits for
 // its own products (with blocks of 128 keys TMEM has room for one buffer, and
-// softmax, P V and the next S of a tile came one after the other). m is raised
+// softmax, P V and the next S of a tile came one after the other). P is rounded
+// to bf16 since V is bf16 and a product's operands have one type: 1.1e-3 rms of O
+// beside the 1.5e-3 of O's own rounding to bf16 (P as two bf16 terms would double
+// the products of P V). Its sum is taken of the fp32 values. m is raised
 // only when a score exceeds it by more than 2^8, so O in TMEM is rarely
 // rescaled.
 //
-// What bounds it: 8 prompts of 4096 with 32 heads take 0.99 ms in a burst
-// (1.1 PFLOP/s) and 1.15 under the power cap; the tensor cores' operands from
+// What bounds it: 8 prompts of 4096 with 32 heads take 1.01 ms in a burst
+// (1.1 PFLOP/s) and 1.13 under the power cap; the tensor cores' operands from
 // shared memory take as long as the products (1280 of about 1660 cycles for 64
-// keys of both tiles). 16 ragged prompts up to 4096, 32 heads on 8: 240 us
-// (0.88 PFLOP/s, clock 1.63 GHz). Short prompts: the longest item's steps.
+// keys of both tiles). 16 ragged prompts up to 4096, 32 heads on 8: 228-231 us
+// (0.93 PFLOP/s, clock 1.67 GHz). Short prompts: the longest item's steps.
 //
 // A sequence may end inside a key block. Keys behind it are masked by the
 // causal mask already; their V rows are zeroed in shared memory before the

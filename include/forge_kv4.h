@@ -69,6 +69,7 @@ int forge_kv4_read(const ForgeKv4* cache, const int32_t* seq, const int32_t* pos
  * probability times its V's scale) of 64 keys to 23 bits of their largest for a
  * head and group of 64 dims, so an output's error is relative to the sum of the
  * weighted rows' largest values in the group (or to 2^-100 where that is less).
+ * A probability below 2^-126 of the largest counts as 0.
  * A scale of V that is NaN or negative, which append does not write, makes the
  * group's output NaN. pos[b] < 0: an
  * empty sequence, its output is zeros (a padded batch). A position beyond the
